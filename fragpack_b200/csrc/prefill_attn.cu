@@ -48,6 +48,7 @@
 #include "fp_api.h"
 #include "fp_common.cuh"
 #include "fp_pipe.cuh"
+#include "fp_tensor.cuh"
 
 namespace fpb {
 namespace {
@@ -66,10 +67,7 @@ constexpr int kRingSlots = 2;  // records alternate K, V: slot 0 serves the K te
 // grew with it in measurement (mean-abs 1.84e-4 at 0, 1.93e-4 at 1, 2.18e-4
 // at 8; max-abs 0.0045, 0.0056, 0.0084), so it is not used.
 constexpr float kRescaleSlack = 0.f;
-constexpr int kTile = 128;
 constexpr int kQTiles = 2;                     // query tiles per CTA, one per warpgroup
-constexpr int kTileBytes = kTile * kTile * 2;  // 32 KB: one operand tile
-constexpr int kHalfTile = kTileBytes / 2;      // one 64-column (128-byte) swizzle atom column
 constexpr uint32_t kTmemColumns = 512;         // S tiles: 0..255, O tiles: 256..511
 
 struct PrefillSmem {
@@ -109,138 +107,6 @@ struct PrefillParams {
   long long wait_limit;
   int skip_page;  // test hook: the decoders do not report this page's K tile (-1: none)
 };
-
-// Byte offset of the 16-byte chunk holding (row, col .. col + 7) of a K-major
-// 128 x 128 BF16 operand tile with the 128-byte swizzle: two column halves of
-// 64 elements, each a stack of 8-row groups of 1024 bytes.
-__device__ __forceinline__ uint32_t tile_chunk(int row, int col) {
-  return (uint32_t)((col >> 6) * kHalfTile + (row >> 3) * 1024 + (row & 7) * 128 +
-                    ((((col & 63) >> 3) ^ (row & 7)) << 4));
-}
-
-// Shared-memory matrix descriptor of an operand tile starting at `addr`
-// (K-major, 128-byte swizzle: 8-row groups 1024 bytes apart).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
-  return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
-
-// Instruction descriptor: BF16 x BF16 -> FP32, both operands K-major, M = N = 128.
-constexpr uint32_t kInstrDesc =
-    (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
-
-__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kInstrDesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-
-// The same with the A operand in tensor memory: 128 rows on the 128 lanes, two
-// BF16 values per 32-bit column, so a K = 16 step spans eight columns.
-__device__ __forceinline__ void umma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                            bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(kInstrDesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-
-// D (+)= A B over the tiles' 128-deep contraction: eight K = 16 steps, each
-// 32 bytes further along the row (four per swizzle atom column).
-__device__ __forceinline__ void tile_product(uint32_t d_tmem, uint32_t a_addr, uint32_t b_addr,
-                                             bool accumulate) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t step = (uint32_t)((j >> 2) * kHalfTile + (j & 3) * 32);
-    umma(d_tmem, tile_desc(a_addr + step), tile_desc(b_addr + step), accumulate || j > 0);
-  }
-}
-
-__device__ __forceinline__ void tile_product_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_addr,
-                                                    bool accumulate) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t step = (uint32_t)((j >> 2) * kHalfTile + (j & 3) * 32);
-    umma_tmem_a(d_tmem, a_tmem + 8u * (uint32_t)j, tile_desc(b_addr + step), accumulate || j > 0);
-  }
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-
-// The same load without the wait: the caller overlaps it with arithmetic on
-// an earlier chunk and calls tmem_wait_loads() before it reads `r`.
-__device__ __forceinline__ void tmem_load32_async(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_loads() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_wait_stores() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
-      "tcgen05.wait::st.sync.aligned;"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
-// No wait inside: the caller calls tmem_wait_stores() once after its last store.
-__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15])
-      : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Decodes one record into an operand tile.  Owner (w, g, c) holds, for word
 // st, the four 8 x 8 pieces (j, f) of rows 16 w + 8 j + 0..7 and columns

@@ -10,6 +10,7 @@ without a CUDA device, the operators raise.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -22,6 +23,7 @@ _DIR = Path(__file__).resolve().parent
 # one compiled with different flags); by default the in-tree library is used.
 LIBRARY = Path(os.environ.get("FRAGPACK_B200_LIBRARY") or _DIR / "libfragpack_b200.so")
 
+_HERE: "contextlib.AbstractContextManager[None]" = contextlib.nullcontext()
 c_i32, c_i64, c_f32, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
 
@@ -68,6 +70,26 @@ class FpPeers(ctypes.Structure):
     ]
 
 
+class FpRotary(ctypes.Structure):
+    """``fp_rotary`` of ``include/fragpack_b200.h``."""
+
+    _fields_ = [("turns", c_ptr), ("rot_dim", c_i32), ("interleaved", c_i32), ("factor", c_f32)]
+
+
+class FpHeads(ctypes.Structure):
+    """``fp_heads`` of ``include/fragpack_b200.h``."""
+
+    _fields_ = [
+        ("input", c_ptr),
+        ("out", c_ptr),
+        ("in_token", c_i64),
+        ("in_head", c_i64),
+        ("out_token", c_i64),
+        ("out_head", c_i64),
+        ("heads", c_i32),
+    ]
+
+
 # name -> argument types; every function returns int.
 _SIGNATURES = {
     "fp_decode_workspace": [c_i32, c_i32, c_ptr, c_ptr, c_ptr],
@@ -84,6 +106,12 @@ _SIGNATURES = {
                                 c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32, c_ptr],
     "fp_prefill_attention": [c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr,
                              c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_ptr, c_ptr],
+    "fp_prompt_attention": [c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i32,
+                            c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32, c_f32, c_ptr],
+    "fp_prompt_status": [c_ptr],
+    "fp_norm_rotary": [c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_i64, c_ptr, c_f32, c_ptr],
+    "fp_hbm_append": [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_ptr,
+                      c_i64, c_ptr, c_f32, c_i32, c_ptr],
     "fp_hbm_prepare": [c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_ptr],
     "fp_hbm_write": [c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i32, c_ptr],
     "fp_hbm_encode": [c_ptr, c_ptr, c_i32, c_ptr, c_i64, c_i64, c_ptr],
@@ -138,9 +166,26 @@ def require_cuda(tensor: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} must be a CUDA tensor: fragpack_b200.ops has no CPU fallback")
 
 
+def on_device(device: torch.device) -> "contextlib.AbstractContextManager[None]":
+    """Make ``device`` current for a launch, if it is not already."""
+    if device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
 def stream_ptr() -> int:
     """Handle of the current CUDA stream."""
     return torch.cuda.current_stream().cuda_stream
 
 
-__all__ = ["EXPORTED", "FpStore", "check", "extension", "require_cuda", "stream_ptr"]
+__all__ = [
+    "EXPORTED",
+    "FpHeads",
+    "FpRotary",
+    "FpStore",
+    "check",
+    "extension",
+    "on_device",
+    "require_cuda",
+    "stream_ptr",
+]

@@ -35,7 +35,8 @@ import torch
 from fragpack_b200.compression import attn_page as ap
 from fragpack_b200.compression.attn_tables import DeviceTables
 from fragpack_b200.logging import init_logger
-from fragpack_b200.ops.fragpack_ext import FpStore, check, extension, stream_ptr
+from fragpack_b200.ops.fragpack_ext import FpStore, check, extension, on_device, stream_ptr
+from fragpack_b200.ops.rotary import Rotary, head_set, rotary_operands
 
 logger = init_logger(__name__)
 
@@ -332,6 +333,73 @@ class HbmKvStore:
                 stream_ptr(),
             )
         )
+
+    def append(
+        self,
+        layer: int,
+        query: torch.Tensor,
+        key: torch.Tensor,
+        value: torch.Tensor,
+        positions: torch.Tensor,
+        slot_mapping: torch.Tensor,
+        rotary: Rotary,
+        query_out: torch.Tensor,
+        key_out: torch.Tensor | None = None,
+        query_weight: torch.Tensor | None = None,
+        key_weight: torch.Tensor | None = None,
+        eps: float = 1e-6,
+    ) -> None:
+        """Norm and rotate one layer's new heads and :meth:`write` its keys and values, one pass.
+
+        ``query`` and ``key`` go through
+        :func:`fragpack_b200.ops.rotary.norm_rotary`; the resulting keys and
+        ``value`` are stored in their blocks' staging.  No counterpart in the
+        reference, whose store is handed rotated keys (``hbm_kv.cu:688-705``).
+
+        Args:
+            layer: Layer index.
+            query: BF16 ``[N, Hq, 128]`` (rows / heads of all heads may be
+                strided by 16-byte multiples).
+            key: BF16 ``[N, H, 128]``.
+            value: BF16 ``[N, H, 128]``.
+            positions: int64 or int32 ``[N]``.
+            slot_mapping: int64 ``[N]`` slot ids, each at most once (negative =
+                not stored; the token's heads are rotated all the same).
+            rotary: The position rotation.
+            query_out: BF16 ``[N, Hq, 128]`` result; may be ``query`` itself.
+            key_out: BF16 ``[N, H, 128]`` to also receive the keys that are
+                stored (what a whole prompt attends to), or None; may be
+                ``key`` itself.
+            query_weight, key_weight: ``[128]`` BF16 or FP32, or None for no norm.
+            eps: Added to the mean square of the norms.
+
+        Raises:
+            RuntimeError: For rejected arguments or a failed launch.
+
+        Async/thread-safety:
+            One kernel on the current stream; CUDA-graph safe.
+        """
+        self._require_device()
+        tokens, device = key.shape[0], self.counters.device
+        q = head_set("query", query, query_out, tokens, device)
+        k = head_set("key", key, key_out, tokens, device)
+        if k.heads != self.kv_heads or value.shape != key.shape or value.stride(2) != 1:
+            raise RuntimeError(f"key and value must be [N, {self.kv_heads}, 128] with a contiguous head dim")
+        if value.dtype != torch.bfloat16 or value.device != device:
+            raise RuntimeError(f"value must be bfloat16 on {device}")
+        if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (tokens,):
+            raise RuntimeError(f"slot_mapping must be int64 [{tokens}]")
+        if not slot_mapping.is_contiguous() or slot_mapping.device != device:
+            raise RuntimeError(f"slot_mapping must be contiguous on {device}")
+        qw, kw, f32, pos, pos64 = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
+        with on_device(device):
+            check(
+                extension().fp_hbm_append(
+                    self._store_ref, ctypes.byref(q), ctypes.byref(k), value.data_ptr(), value.stride(0),
+                    value.stride(1), qw, kw, f32, pos, pos64, slot_mapping.data_ptr(), tokens,
+                    ctypes.byref(rotary._native), float(eps), layer, stream_ptr(),
+                )
+            )
 
     def encode(self, layer: int, max_close: int) -> None:
         """Code this layer's records of every block closed this step.

@@ -1,0 +1,95 @@
+"""Causal attention of packed whole prompts over BF16 keys and values (sm_100a, tcgen05).
+
+A prompt's first prefill step attends only to keys and values that the same
+step has just produced.  :func:`prompt_attention` reads them where they are,
+in the layer's projection, instead of the store: no record is decoded and no
+workspace is filled (the reference sends such a step through ``store.gather``
+and FlashAttention like any other, ``fragpack/integrations/vllm/backend.py:560-575``;
+:func:`fragpack_b200.ops.prefill_attn.prefill_attention` serves the steps that
+also see cached blocks).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from fragpack_b200.ops.fragpack_ext import check, extension, on_device, require_cuda, stream_ptr
+from fragpack_b200.ops.fused_attn_decode import GQA
+
+PROMPT_WAIT_TIMEOUT = 1
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    starts: torch.Tensor,
+    scale: float,
+    out: torch.Tensor,
+) -> None:
+    """Attend every prompt's tokens over itself, causally.
+
+    Prompt ``r`` owns the rows ``starts[r] .. starts[r + 1]`` of all four
+    tensors; each of its rows sees the prompt's rows up to and including
+    itself.  Rows outside every prompt are left as they were, and what they
+    hold reaches no result.
+
+    Args:
+        q: BF16 ``[T, H * G, 128]`` queries.
+        k, v: BF16 ``[T, H, 128]`` keys and values.  Tokens and heads of all
+            tensors may be strided by 16-byte multiples.
+        starts: int32 ``[R + 1]`` first row of each prompt, non-decreasing;
+            entries are clamped to ``0 .. T``.
+        scale: Softmax scale, positive.
+        out: BF16 ``[T, H * G, 128]`` output; must not overlap the inputs.
+
+    Raises:
+        ValueError: If the query group does not divide ``GQA``.
+        RuntimeError: For rejected arguments or a failed launch.
+
+    Async/thread-safety:
+        One kernel on the current CUDA stream; CUDA-graph safe; allocates nothing.
+    """
+    require_cuda(q, "q")
+    if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0:
+        raise RuntimeError("q, k and v must be [T, heads, 128]")
+    tokens, kv_heads = k.shape[0], k.shape[1]
+    group = q.shape[1] // kv_heads
+    if group == 0 or group * kv_heads != q.shape[1] or GQA % group:
+        raise ValueError(f"query heads {q.shape[1]} need a group dividing {GQA}")
+    if k.shape != (tokens, kv_heads, 128) or v.shape != k.shape or q.shape[0] != tokens or q.shape[2] != 128:
+        raise RuntimeError("q must be [T, H * G, 128] and k, v [T, H, 128]")
+    if out.shape != q.shape:
+        raise RuntimeError("out must have the shape of q")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        if t.dtype != torch.bfloat16 or t.device != q.device or t.stride(2) != 1:
+            raise RuntimeError(f"{name} must be bfloat16 on {q.device} with a contiguous head dim")
+    if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() == 0 or not starts.is_contiguous():
+        raise RuntimeError("starts must be contiguous int32 [R + 1]")
+    if starts.device != q.device:
+        raise RuntimeError(f"starts must be on {q.device}")
+    with on_device(q.device):
+        check(
+            extension().fp_prompt_attention(
+                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                v.stride(0), v.stride(1), starts.data_ptr(), starts.numel() - 1, tokens, out.data_ptr(),
+                out.stride(0), out.stride(1), kv_heads, group, float(scale), stream_ptr(),
+            )
+        )
+
+
+def prompt_status() -> int:
+    """Status word of the prompt kernel on the current device (synchronises) and clear it.
+
+    Returns:
+        0, or ``PROMPT_WAIT_TIMEOUT`` if a bounded device-side wait ran out
+        since the last read (the outputs of those calls are invalid).
+    """
+    word = ctypes.c_int32(0)
+    check(extension().fp_prompt_status(ctypes.byref(word)))
+    return int(word.value)
+
+
+__all__ = ["PROMPT_WAIT_TIMEOUT", "prompt_attention", "prompt_status"]

@@ -1,0 +1,273 @@
+"""Norms of query and key heads with the position rotation, one pass (sm_100a).
+
+What a decoder layer does to its projected heads before they meet the cache:
+an optional RMS norm of every query and key head and the rotation by the
+token's position.  :func:`norm_rotary` does it for callers that hand rotated
+heads to the attention backend (whose ``forward`` writes the keys itself, as
+the reference's, ``fragpack/integrations/vllm/backend.py:504-579``);
+``HbmKvStore.append`` does the same on the way into the store.  The reference
+has no counterpart: its engine rotates before the backend is called.
+
+A :class:`Rotary` holds the frequencies in turns per token as 64-bit binary
+fractions, so that ``position * frequency`` modulo one turn is exact at any
+position and no table of angles is kept.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+import math
+from typing import Any
+
+import numpy as np
+import torch
+
+from fragpack_b200.ops.fragpack_ext import (
+    FpHeads,
+    FpRotary,
+    check,
+    extension,
+    on_device,
+    require_cuda,
+    stream_ptr,
+)
+
+HEAD_DIM = 128
+
+
+def rotary_frequencies(
+    rot_dim: int = HEAD_DIM, base: float = 10000.0, scaling: dict[str, Any] | None = None
+) -> tuple[np.ndarray, float]:
+    """Frequencies of the rotated pairs and the factor on the rotated dims.
+
+    Pair ``i`` turns by ``base ** (-2 i / rot_dim)`` radians per token.  For
+    contexts longer than the model was trained on, ``scaling`` names a rule:
+
+    * ``{"type": "linear", "factor"}``: every frequency divided by ``factor``
+      (positions interpolated);
+    * ``{"type": "bands", "factor", "low_freq_factor", "high_freq_factor",
+      "original"}``: pairs that turn at least ``high_freq_factor`` times over
+      the ``original`` context keep their frequency, those that turn at most
+      ``low_freq_factor`` times are divided by ``factor``, linear in the
+      number of turns in between;
+    * ``{"type": "ramp", "factor", "original", "beta_fast", "beta_slow"}``:
+      the same idea, linear in the pair's index between the pairs that turn
+      ``beta_fast`` (default 32) and ``beta_slow`` (default 1) times, and the
+      rotated dims are multiplied by ``"attention_factor"`` (default
+      ``0.1 ln(factor) + 1``).
+
+    Args:
+        rot_dim: Rotated dims, even.
+        base: Base of the geometric progression.
+        scaling: A rule as above, or None.
+
+    Returns:
+        float64 ``[rot_dim / 2]`` radians per token, and the factor.
+
+    Raises:
+        ValueError: For an unknown rule or impossible parameters.
+    """
+    if rot_dim < 0 or rot_dim % 2 or base <= 1.0:
+        raise ValueError(f"rotated dims {rot_dim} must be even and the base {base} above 1")
+    freq = base ** (-np.arange(0, rot_dim, 2, dtype=np.float64) / max(rot_dim, 1))
+    if scaling is None:
+        return freq, 1.0
+    rule, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
+    if rule not in ("linear", "bands", "ramp"):
+        raise ValueError(f"unknown rotary scaling {rule!r}")
+    if not factor >= 1.0:
+        raise ValueError(f"rotary scaling needs a factor of at least 1, not {factor}")
+    if rule == "linear":
+        return freq / factor, 1.0
+    original = float(scaling["original"])
+    if rule == "bands":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not high > low:
+            raise ValueError("rotary bands need high_freq_factor above low_freq_factor")
+        turns = original * freq / (2.0 * math.pi)
+        keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        return freq * keep + freq / factor * (1.0 - keep), 1.0
+
+    def pair_turning(times: float) -> float:
+        return rot_dim * math.log(original / (2.0 * math.pi * times)) / (2.0 * math.log(base))
+
+    first = max(math.floor(pair_turning(float(scaling.get("beta_fast", 32.0)))), 0)
+    last = min(math.ceil(pair_turning(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    ramp = np.clip((np.arange(rot_dim // 2) - first) / max(last - first, 1e-3), 0.0, 1.0)
+    attention = float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
+    return freq * (1.0 - ramp) + freq / factor * ramp, attention
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """A position rotation on one device (see :func:`make_rotary`).
+
+    Attributes:
+        turns: int64 ``[rot_dim / 2]`` CUDA tensor: turns per token as 64-bit
+            binary fractions (the bits of unsigned integers).
+        rot_dim: Rotated dims of a head, a multiple of 8 up to 128.
+        interleaved: Pairs are dims ``(2 i, 2 i + 1)`` instead of
+            ``(i, i + rot_dim / 2)``.
+        factor: Multiplies the rotated dims.
+    """
+
+    turns: torch.Tensor
+    rot_dim: int
+    interleaved: bool
+    factor: float
+    _native: FpRotary = field(repr=False, compare=False)
+
+
+def make_rotary(
+    device: torch.device,
+    rot_dim: int = HEAD_DIM,
+    base: float = 10000.0,
+    interleaved: bool = False,
+    scaling: dict[str, Any] | None = None,
+    frequencies: Any = None,
+    factor: float | None = None,
+) -> Rotary:
+    """Build a :class:`Rotary` on ``device``.
+
+    Args:
+        device: Where the heads live.
+        rot_dim: Rotated dims, a multiple of 8 up to 128 (0: no rotation);
+            further dims of a head stay as they are.
+        base, scaling: See :func:`rotary_frequencies`.
+        interleaved: Layout of the pairs.
+        frequencies: Radians per token ``[rot_dim / 2]``, in place of those of
+            ``base`` and ``scaling``.
+        factor: Factor on the rotated dims, in place of the rule's.
+
+    Raises:
+        ValueError: For impossible parameters.
+    """
+    if rot_dim < 0 or rot_dim > HEAD_DIM or rot_dim % 8:
+        raise ValueError(f"rotated dims {rot_dim} must be a multiple of 8 up to {HEAD_DIM}")
+    if frequencies is None:
+        freq, rule_factor = rotary_frequencies(rot_dim, base, scaling)
+    else:
+        if isinstance(frequencies, torch.Tensor):
+            frequencies = frequencies.detach().cpu().to(torch.float64).numpy()
+        freq = np.asarray(frequencies, dtype=np.float64)
+        rule_factor = 1.0
+        if freq.shape != (rot_dim // 2,) or not np.isfinite(freq).all():
+            raise ValueError(f"frequencies must be {rot_dim // 2} finite numbers")
+    factor = float(rule_factor if factor is None else factor)
+    # The fraction of a turn per token; whole turns per token change nothing.
+    fractions = [int(f / (2.0 * math.pi) * 2.0**64) % (1 << 64) for f in freq.tolist()]
+    bits = np.array(fractions + [0] * (not fractions), dtype=np.uint64).view(np.int64)
+    turns = torch.from_numpy(bits).to(device)
+    native = FpRotary(turns=turns.data_ptr(), rot_dim=rot_dim, interleaved=int(bool(interleaved)), factor=factor)
+    return Rotary(turns, rot_dim, bool(interleaved), factor, native)
+
+
+def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: torch.device) -> FpHeads:
+    """Check one set of heads and its result and describe them to the library."""
+    if heads.dim() != 3 or heads.shape[2] != HEAD_DIM or heads.stride(2) != 1:
+        raise RuntimeError(f"{name} must be [T, heads, {HEAD_DIM}] with a contiguous head dim")
+    if heads.shape[0] != tokens:
+        raise RuntimeError(f"{name} has {heads.shape[0]} tokens, not {tokens}")
+    if heads.dtype != torch.bfloat16 or heads.device != device:
+        raise RuntimeError(f"{name} must be bfloat16 on {device}")
+    if out is None:
+        return FpHeads(heads.data_ptr(), None, heads.stride(0), heads.stride(1), 0, 0, heads.shape[1])
+    if out.shape != heads.shape or out.stride(2) != 1:
+        raise RuntimeError(f"{name}_out must have the shape of {name} and a contiguous head dim")
+    if out.dtype != torch.bfloat16 or out.device != device:
+        raise RuntimeError(f"{name}_out must be bfloat16 on {device}")
+    return FpHeads(heads.data_ptr(), out.data_ptr(), heads.stride(0), heads.stride(1), out.stride(0),
+                   out.stride(1), heads.shape[1])
+
+
+def rotary_operands(
+    positions: torch.Tensor,
+    tokens: int,
+    rotary: Rotary,
+    query_weight: torch.Tensor | None,
+    key_weight: torch.Tensor | None,
+    device: torch.device,
+) -> tuple[int | None, int | None, int, int, int]:
+    """Check what :func:`norm_rotary` and ``HbmKvStore.append`` share.
+
+    Returns:
+        Pointers of the two weights, whether they are FP32, the pointer of the
+        positions and whether those are int64.
+    """
+    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,):
+        raise RuntimeError(f"positions must be int64 or int32 [{tokens}]")
+    if not positions.is_contiguous() or positions.device != device or rotary.turns.device != device:
+        raise RuntimeError(f"positions must be contiguous and on {device}, like the rotary's frequencies")
+    dtype = None
+    for weight in (query_weight, key_weight):
+        if weight is None:
+            continue
+        if weight.dtype not in (torch.bfloat16, torch.float32) or weight.dtype != (dtype or weight.dtype):
+            raise RuntimeError("norm weights must both be bfloat16 or both float32")
+        if weight.shape != (HEAD_DIM,) or not weight.is_contiguous() or weight.device != device:
+            raise RuntimeError(f"norm weights must be contiguous [{HEAD_DIM}] on {device}")
+        dtype = weight.dtype
+    return (
+        None if query_weight is None else query_weight.data_ptr(),
+        None if key_weight is None else key_weight.data_ptr(),
+        int(dtype == torch.float32),
+        positions.data_ptr(),
+        int(positions.dtype == torch.int64),
+    )
+
+
+_NO_HEADS = FpHeads(None, None, 0, 0, 0, 0, 0)
+
+
+def norm_rotary(
+    query: torch.Tensor,
+    key: torch.Tensor | None,
+    positions: torch.Tensor,
+    rotary: Rotary,
+    query_out: torch.Tensor,
+    key_out: torch.Tensor | None,
+    query_weight: torch.Tensor | None = None,
+    key_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> None:
+    """RMS norm of every query and key head, then the position rotation.
+
+    A head ``x`` becomes ``x * rsqrt(mean(x^2) + eps) * weight`` (left out
+    without a weight), in FP32, and its pairs are rotated by ``position *
+    frequency``; the result is rounded to BF16 once.
+
+    Args:
+        query: BF16 ``[T, Hq, 128]`` (tokens and heads may be strided by
+            16-byte multiples, as the slices of a packed projection are).
+        key: BF16 ``[T, H, 128]``, or None for queries alone.
+        positions: int64 or int32 ``[T]``.
+        rotary: The rotation.
+        query_out, key_out: BF16 results of the same shapes; may be ``query``
+            / ``key`` themselves, must not overlap the inputs otherwise.
+        query_weight, key_weight: ``[128]`` BF16 or FP32, or None for no norm.
+        eps: Added to the mean square.
+
+    Raises:
+        RuntimeError: For rejected arguments or a failed launch.
+
+    Async/thread-safety:
+        One kernel on the current CUDA stream; CUDA-graph safe; allocates nothing.
+    """
+    require_cuda(query, "query")
+    if (key is None) != (key_out is None):
+        raise RuntimeError("key and key_out come together")
+    device, tokens = query.device, query.shape[0]
+    q = head_set("query", query, query_out, tokens, device)
+    k = _NO_HEADS if key is None else head_set("key", key, key_out, tokens, device)
+    operands = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
+    with on_device(device):
+        check(
+            extension().fp_norm_rotary(
+                ctypes.byref(q), ctypes.byref(k), *operands, tokens, ctypes.byref(rotary._native), float(eps),
+                stream_ptr(),
+            )
+        )
+
+
+__all__ = ["Rotary", "make_rotary", "norm_rotary", "rotary_frequencies"]

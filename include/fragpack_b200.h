@@ -254,6 +254,80 @@ int fp_prefill_attention(const void* q, int64_t q_stride, const int64_t* rec_add
                          int32_t max_query_tokens, int32_t kv_heads, int32_t group, float scale,
                          int32_t* status, void* stream);
 
+/*
+ * Causal attention of packed whole prompts over the BF16 keys and values at
+ * hand (no counterpart in the reference, whose first prefill chunk also goes
+ * through store.gather and flash_attn_varlen_func,
+ * fragpack/integrations/vllm/backend.py:560-575).  Prompt r owns the rows
+ * starts[r] .. starts[r + 1] of q, k, v and out; row i of it attends rows up to
+ * and including itself.
+ *
+ *   q, out      BF16 [tokens, kv_heads * group, 128]; token and head strides in
+ *               scalars, multiples of 8 and positive, rows 16-byte aligned
+ *   k, v        BF16 [tokens, kv_heads, 128], strides as q
+ *   starts      int32 [prompts + 1], non-decreasing, within 0 .. tokens; rows
+ *               outside are neither attended nor written
+ *   group       query heads per KV head: 1, 2, 4 or 8
+ *   scale       softmax scale, > 0
+ * Its device-side waits are bounded; should one run out, bit 0 of the status
+ * word read by fp_prompt_status is set (the outputs are then invalid).
+ */
+int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                        int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                        int64_t v_head, const int32_t* starts, int32_t prompts, int64_t tokens,
+                        void* out, int64_t o_token, int64_t o_head, int32_t kv_heads, int32_t group,
+                        float scale, void* stream);
+
+/* Copies the prompt kernel's status word to the host (synchronises the device's
+ * prior work on the legacy stream) and clears it. */
+int fp_prompt_status(int32_t* status);
+
+/*
+ * A position rotation: `turns` holds, for each of the rot_dim / 2 pairs, the
+ * rotation per token in turns as a 64-bit binary fraction (device memory,
+ * 16-byte aligned); rot_dim is a multiple of 8 up to 128 (0: none), further
+ * dims stay as they are.  Pairs are dims (i, i + rot_dim / 2), or
+ * (2 i, 2 i + 1) if `interleaved`; `factor` multiplies the rotated dims.
+ */
+typedef struct fp_rotary {
+  const uint64_t* turns;
+  int32_t rot_dim, interleaved;
+  float factor;
+} fp_rotary;
+
+/* Heads BF16 [tokens, heads, 128] and where their results go (may be `in`
+ * itself; otherwise the two must not overlap); strides in scalars, multiples of
+ * 8, rows 16-byte aligned. */
+typedef struct fp_heads {
+  const void* in;
+  void* out;
+  int64_t in_token, in_head, out_token, out_head;
+  int32_t heads;
+} fp_heads;
+
+/*
+ * RMS norm of every query and key head and the position rotation, one pass (no
+ * counterpart in the reference, whose backend receives rotated heads).
+ *   q_weight/k_weight  [128] BF16, or FP32 if weights_f32; null: no norm
+ *   positions   int32 [tokens], or int64 if positions_64
+ * Either set of heads may be empty (heads = 0).
+ */
+int fp_norm_rotary(const fp_heads* q, const fp_heads* k, const void* q_weight, const void* k_weight,
+                   int32_t weights_f32, const void* positions, int32_t positions_64, int64_t tokens,
+                   const fp_rotary* rotary, float eps, void* stream);
+
+/*
+ * fp_norm_rotary and fp_hbm_write in one pass: the rotated keys and the values
+ * (BF16 [tokens, H, 128]) go to their blocks' staging, the rotated queries to
+ * q->out and, where k->out is not null, the rotated keys also there.  A token
+ * with a negative slot is not stored, but its heads are rotated all the same.
+ */
+int fp_hbm_append(const fp_store* store, const fp_heads* q, const fp_heads* k, const void* value,
+                  int64_t v_stride0, int64_t v_stride1, const void* q_weight, const void* k_weight,
+                  int32_t weights_f32, const void* positions, int32_t positions_64,
+                  const int64_t* slot_mapping, int64_t tokens, const fp_rotary* rotary, float eps,
+                  int32_t layer, void* stream);
+
 /* hbm_prepare (fragpack/ops/hbm_kv.cu:669-686): start a step. */
 int fp_hbm_prepare(const fp_store* store, const int64_t* slot_mapping, int64_t num_tokens,
                    const int32_t* live, int64_t num_live, int32_t step, void* stream);
