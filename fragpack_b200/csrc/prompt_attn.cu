@@ -3,23 +3,39 @@
 //
 //   o_i = sum_{j <= i} p_ij v_j / sum_{j <= i} p_ij,   p_ij = exp(scale q_i . k_j - m_i)
 //
-// A CTA takes two tiles of 128 query rows of one KV head (a row is a token and
-// a query head of the group: 128 / G tokens x G heads), walks the prompt's keys
-// in tiles of 128 and runs both products on the tensor cores (tcgen05.mma):
+// An item is two tiles of 128 query rows of one KV head (a row is a token and a
+// query head of the group: 128 / G tokens x G heads).  It walks the prompt's
+// keys in tiles of kKeys and runs both products on the tensor cores:
 //
 //   S = Q K^T      A = Q tile, B = K tile, both [rows, 128 dims], K-major
-//   O += P V       A = P in tensor memory, B = V tile [128 tokens, 128 dims], MN-major
+//   O += P V       A = P in tensor memory, B = V tile [kKeys tokens, 128 dims], MN-major
 //
 // Every tile is brought by TMA (128-byte swizzle) straight from the packed
 // projection, whatever its strides.  Running maximum and sum of the softmax are
-// FP32, one thread per query row; P is rounded to BF16 for the second product
-// and the denominator sums the unrounded values, as in decode attention.
+// FP32; P is rounded to BF16 for the second product and the denominator sums
+// the unrounded values, as in decode attention.
 //
-//   warps 0-3   softmax of query tile 0, warps 4-7 of query tile 1
-//   warp 8      issues every tcgen05.mma
-//   warp 9      TMA loads
+// Tensor memory holds two O tiles (256 columns), two S tiles (2 kKeys) and P.  P
+// has columns of its own, so that the next scores of a tile are made while the
+// softmax works on these; a tile's chain is then the softmax alone, and the
+// tensor cores follow.  That is why a key tile is narrower than 128: with 128
+// keys P has to lie over its S, every tile waits for softmax, O product and S
+// product in turn, and the same kernel took 3,800 cycles per 128 keys of an item
+// against 2,048 of the products.
+//
+// One persistent CTA per SM; its warps meet only through mbarriers, and every
+// wait is bounded and reports through the status word:
+//   softmax warps  those of query tile 0, then those of tile 1 (a warp reaches
+//                  the tensor-memory lanes 32 (warp % 4) ..)
+//   result warps   divide an item's O by the sums and store it
+//   score warp     issues S products, value warp O products (one elected lane;
+//                  two warps, so that neither waits behind the other's barriers)
+//   load warp      picks the CTA's items and loads their tiles
 #include <cuda.h>
 #include <math.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "fp_api.h"
 #include "fp_common.cuh"
@@ -30,24 +46,51 @@ namespace fpb {
 namespace {
 
 constexpr int kQTiles = 2;
-constexpr int kStages = 2;            // K tiles and V tiles in flight, each
-constexpr int kSoftmaxThreads = 256;  // one warpgroup per query tile, thread = row
-constexpr int kIssueWarp = 8, kLoadWarp = 9;
-constexpr int kPromptThreads = kSoftmaxThreads + 64;
-constexpr uint32_t kTmemColumns = 512;  // S tiles: 0..255, O tiles: 256..511
+constexpr int kKeys = 80;                  // keys of a tile
+constexpr int kParts = 1;                  // softmax threads of a query row
+constexpr int kStages = 3;                 // K tiles and V tiles in flight, each
+constexpr int kKeyTileBytes = kKeys * 256;
+constexpr int kKeyHalf = kKeys * 128;      // one 64-dim half of a K or V tile
+constexpr int kSoftmaxWarps = 8 * kParts, kResultWarps = 4;
+constexpr int kScoreWarp = kSoftmaxWarps + kResultWarps, kValueWarp = kScoreWarp + 1, kLoadWarp = kScoreWarp + 2;
+constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kResultWarps + 4);  // whole warpgroups
+constexpr int kItemReaders = kValueWarp + 1;  // warps that read an item's description
+// Tensor memory columns: O tiles, S tiles, P tiles.
+constexpr uint32_t kTmemColumns = 512, kTmemS = kQTiles * kTile, kTmemP = kTmemS + kQTiles * kKeys;
+static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "tensor memory is full");
+// Registers of the softmax warps, of the result warps and of the rest; together
+// what the block is launched with.
+constexpr int kSoftmaxRegs = kParts == 1 ? 184 : 96, kResultRegs = kParts == 1 ? 88 : 56,
+              kOtherRegs = kParts == 1 ? 56 : 40;
+// How far (log2 units) a row's maximum may rise above the reference point of its
+// exponentials before the reference follows and O is rescaled.
+constexpr float kRescaleSlack = 8.f;
 
 __device__ int32_t g_prompt_status;
 
+// What every role needs to know about an item.
+struct Item {
+  int head, row0, length;  // KV head, first row and rows (tokens) of the prompt
+  int tok0;                // first token of query tile 0
+  int last[kQTiles];       // last key tile of each query tile; -1: it has no rows
+};
+
 struct PromptSmem {
   __align__(1024) uint8_t q[kQTiles][kTileBytes];
-  __align__(1024) uint8_t k[kStages][kTileBytes];
-  __align__(1024) uint8_t v[kStages][kTileBytes];
-  __align__(8) uint64_t q_full;
+  __align__(1024) uint8_t k[kStages][kKeyTileBytes];
+  __align__(1024) uint8_t v[kStages][kKeyTileBytes];
+  float sum[kQTiles][kTile];             // of the probabilities of each row
+  float half_row[2][kQTiles][2][kTile];  // what the two softmax threads of a row exchange
+  Item item[2];
+  __align__(8) uint64_t item_full[2], item_empty[2];
+  uint64_t q_full[kQTiles], q_empty[kQTiles];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_ready[kQTiles], p_ready[kQTiles], o_done[kQTiles];
-  uint64_t drained;
+  uint64_t s_ready[kQTiles], s_free[kQTiles];         // S product done; S read
+  uint64_t p_ready[kQTiles], p_free[kQTiles];         // P written and O rescaled; O product done
+  uint64_t sum_full[kQTiles], sum_empty[kQTiles];
+  uint64_t o_done[kQTiles], o_free[kQTiles];          // the item's last O product done; O read
+  uint64_t drained[2];
   uint32_t tmem_base;
-  int row0, length, tile;  // of the CTA's work; tile -1: none
   WaitState wait;
 };
 
@@ -63,51 +106,135 @@ struct PromptParams {
   __nv_bfloat16* out;
   int64_t o_token, o_head;
   const int32_t* starts;
-  int prompts, tokens, group;
+  int prompts, tokens, kv_heads, group;
   float scale_log2;
   long long wait_limit;
-  int skip_tile;  // test hook: this K tile is not loaded (-1: none)
+  int skip_tile;  // test hook: this K tile of an item is not loaded (-1: none)
 };
 
-// What every role needs to know about the CTA's work.
-struct PromptWork {
-  int head, row0, length;  // KV head, first row and rows (tokens) of the prompt
-  int tok0, tile_tokens;   // first token of tile 0, tokens per tile
-  int last[kQTiles];       // last key tile of each query tile; -1: it has no rows
-  int last_any;
-};
+// As bounded_wait, inlined whole (a call would keep the register split from
+// taking effect) and without a suspend-time hint: with hints of 2 and 20
+// microseconds the waits woke later and the kernel took a tenth longer.
+__device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, WaitState* ws) {
+  if (arrived(bar, parity)) return true;
+  volatile int* abort = &ws->abort;
+  const long long t0 = clock64();
+#pragma unroll 1
+  while (!*abort) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (arrived(bar, parity)) return true;
+    if (clock64() - t0 > ws->limit) {
+      *abort = 1;
+      atomicOr(ws->status, FP_DECODE_WAIT_TIMEOUT);
+    }
+  }
+  return false;
+}
 
-// Key tile coordinates: {dim, head, token}.
+__device__ __forceinline__ void tmem_acquire() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_release() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// Tile coordinates: {dim, head, token}.
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
       : "memory");
 }
-
-// V tile as the B operand: rows are the contraction (tokens), 64 dims side by
-// side: groups of 8 tokens 1024 bytes apart, the two halves of the dims
-// kHalfTile apart (MN-major, 128-byte swizzle).
-__device__ __forceinline__ uint64_t value_desc(uint32_t addr) {
-  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(kHalfTile >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+template <int kRows>
+__device__ __forceinline__ void tma_load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
+  mbar_expect_tx(bar, kRows * 256);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) tma_load(dst + h * kRows * 128, map, 64 * h, head, row, bar);
 }
+
+// The low words of the operand descriptors (address / 16); the rest is constant.
+// K-major (Q, K): groups of 8 rows 1024 bytes apart, as tile_desc.  MN-major
+// (V: rows are the contraction, 64 dims side by side): groups of 8 tokens 1024
+// bytes apart, the two halves of the dims kKeyHalf apart.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t key_desc_low(uint32_t addr) { return ((addr & 0x3ffffu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t value_desc_low(uint32_t addr) {
+  return ((addr & 0x3ffffu) >> 4) | ((uint32_t)(kKeyHalf >> 4) << 16);
+}
+constexpr uint32_t kScoreInstr = (kInstrDesc & ~(63u << 17)) | ((uint32_t)(kKeys >> 3) << 17);  // N = kKeys
 constexpr uint32_t kValueInstr = kInstrDesc | (1u << 16);  // B is MN-major
 
-// O (+)= P V over 128 tokens: eight steps of 16 tokens, 2048 bytes apart in V
-// and eight tensor-memory columns apart in P.
-__device__ __forceinline__ void value_product(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_addr, bool accumulate) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    umma_tmem_a(d_tmem, p_tmem + 8u * (uint32_t)j, value_desc(v_addr + 2048u * (uint32_t)j), accumulate || j > 0,
-                kValueInstr);
+// The products of one pair of tiles, in steps of 16, by one elected lane
+// (the whole warp calls).  One block of assembly: written instruction by
+// instruction, moving each descriptor to the uniform registers that the
+// instruction reads took longer (90 cycles) than the product itself (64).
+#define FP_STEP(a_off, b_off, acc)            \
+  "add.u32 a, %1, " #a_off ";\n\t"            \
+  "add.u32 b, %2, " #b_off ";\n\t"            \
+  "mov.b64 da, {a, %3};\n\t"                  \
+  "mov.b64 db, {b, %3};\n\t"                  \
+  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, " acc ";\n\t"
+
+// S = Q K^T: the 128-deep rows are two halves of four steps of 32 bytes.
+__device__ __forceinline__ void score_product(uint32_t d_tmem, uint32_t q_low, uint32_t k_low) {
+  asm volatile(
+      "{\n\t.reg .pred q, no, yes;\n\t.reg .b32 a, b;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 no, 0, 0;\n\tsetp.eq.b32 yes, 0, 0;\n\t"
+      FP_STEP(0, 0, "no") FP_STEP(2, 2, "yes") FP_STEP(4, 4, "yes") FP_STEP(6, 6, "yes")
+      "add.u32 %2, %2, %5;\n\t"
+      FP_STEP(1024, 0, "yes") FP_STEP(1026, 2, "yes") FP_STEP(1028, 4, "yes") FP_STEP(1030, 6, "yes")
+      "}"
+      : "+r"(d_tmem), "+r"(q_low), "+r"(k_low)
+      : "n"(kDescHigh), "r"(kScoreInstr), "n"(kKeyHalf / 16)
+      : "memory");
+}
+#undef FP_STEP
+
+// O (+)= P V over kKeys tokens: steps of 16 tokens, 2048 bytes apart in V and
+// eight tensor-memory columns apart in P.
+#define FP_STEP(a_off, b_off, acc)            \
+  "add.u32 a, %1, " #a_off ";\n\t"            \
+  "add.u32 b, %2, " #b_off ";\n\t"            \
+  "mov.b64 db, {b, %3};\n\t"                  \
+  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, " acc ";\n\t"
+__device__ __forceinline__ void value_product(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_low, bool accumulate) {
+  static_assert(kKeys == 80, "the steps below");
+  asm volatile(
+      "{\n\t.reg .pred q, acc, yes;\n\t.reg .b32 a, b;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 acc, %5, 0;\n\tsetp.eq.b32 yes, 0, 0;\n\t"
+      FP_STEP(0, 0, "acc") FP_STEP(8, 128, "yes") FP_STEP(16, 256, "yes") FP_STEP(24, 384, "yes")
+      FP_STEP(32, 512, "yes")
+      "}"
+      ::"r"(d_tmem), "r"(p_tmem), "r"(v_low), "n"(kDescHigh), "r"(kValueInstr), "r"((uint32_t)accumulate)
+      : "memory");
+}
+#undef FP_STEP
+
+// Arrives on `bar` when everything issued so far is done; one elected lane, the
+// same as above, where `wanted`.
+__device__ __forceinline__ void commit(uint64_t* bar, bool wanted = true) {
+  asm volatile(
+      "{\n\t.reg .pred q, w;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 w, %1, 0;\n\tand.pred q, q, w;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_addr(bar)), "r"((uint32_t)wanted)
+      : "memory");
 }
 
-// One warp finds the CTA's prompt: item x of the list of all prompts' pairs of
-// query tiles, the last (longest) pair of each prompt first.
-__device__ __forceinline__ void find_work(const PromptParams& p, PromptSmem& sm, int lane) {
-  const int pair_tokens = kQTiles * kTile / p.group;
-  int left = (int)blockIdx.x;
+// ---------------------------------------------------------------------------
+// Items.  Item x of a KV head is a pair of query tiles of some prompt; pair i of
+// a prompt costs the more the larger i is, and the same in every prompt.
+
+// One lane per prompt, 32 at a time: f(prompt index, first row, rows) of every
+// prompt, in order; stops when f returns true (f is warp-uniform).
+template <typename F>
+__device__ __forceinline__ void each_prompts(const PromptParams& p, int lane, F&& f) {
+#pragma unroll 1
   for (int base = 0; base < p.prompts; base += 32) {
     const int r = base + lane;
     int row0 = 0, length = 0;
@@ -115,168 +242,432 @@ __device__ __forceinline__ void find_work(const PromptParams& p, PromptSmem& sm,
       row0 = max(0, min(p.starts[r], p.tokens));
       length = max(0, min(p.starts[r + 1], p.tokens) - row0);
     }
-    const int pairs = (length + pair_tokens - 1) / pair_tokens;
-    int upto = pairs;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += other;
+    if (f(row0, length)) return;
+  }
+}
+
+// Finds item x of the order "all prompts' pairs i, from the largest i down";
+// false: there are fewer.  The whole warp calls; every lane gets the result.
+__device__ __forceinline__ bool find_item(const PromptParams& p, int x, int lane, int& row0, int& length, int& pair) {
+  const int pair_tokens = kQTiles * kTile / p.group;
+  const auto pairs_of = [&](int rows) { return (rows + pair_tokens - 1) / pair_tokens; };
+  // Pairs with index >= level, over all prompts.
+  const auto pairs_from = [&](int level) {
+    int count = 0;
+    each_prompts(p, lane, [&](int, int rows) {
+      count += (int)__reduce_add_sync(0xffffffffu, (unsigned)max(0, pairs_of(rows) - level));
+      return false;
+    });
+    return count;
+  };
+  if (x >= pairs_from(0)) return false;
+  int low = 0, high = (p.tokens + pair_tokens - 1) / pair_tokens;  // pairs_from(low) > x >= pairs_from(high)
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (pairs_from(mid) > x) low = mid; else high = mid;
+  }
+  pair = low;
+  int rank = x - pairs_from(low + 1);
+  each_prompts(p, lane, [&](int first, int rows) {
+    const uint32_t have = __ballot_sync(0xffffffffu, pairs_of(rows) > low);
+    const int count = __popc(have);
+    if (rank >= count) {
+      rank -= count;
+      return false;
     }
-    const uint32_t beyond = __ballot_sync(0xffffffffu, upto > left);
-    if (beyond) {
-      if (lane == __ffs(beyond) - 1) {
-        sm.row0 = row0;
-        sm.length = length;
-        sm.tile = pairs - 1 - (left - (upto - pairs));
+    const int src = __fns(have, 0, rank + 1);
+    row0 = __shfl_sync(0xffffffffu, first, src);
+    length = __shfl_sync(0xffffffffu, rows, src);
+    return true;
+  });
+  return true;
+}
+
+__device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& sm, int lane) {
+  const int tile_tokens = kTile / p.group;
+  int q_used[kQTiles] = {0, 0};
+  int tiles = 0;  // key tiles loaded by this CTA so far
+  bool ok = true;
+  for (int n = 0;; ++n) {
+    const int slot = n & 1;
+    // CTAs take items forwards and backwards in turn, so that the sums of what
+    // they get stay close.
+    const int64_t at = (int64_t)n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    const int head = (int)(at % p.kv_heads);
+    Item w;
+    int pair = 0;
+    const bool more = at / p.kv_heads < (1 << 30) &&
+                      find_item(p, (int)(at / p.kv_heads), lane, w.row0, w.length, pair);
+    w.head = more ? head : -1;
+    w.tok0 = pair * kQTiles * tile_tokens;
+#pragma unroll
+    for (int t = 0; t < kQTiles; ++t) {
+      const int t0 = w.tok0 + t * tile_tokens;
+      w.last[t] = more && t0 < w.length ? (min(t0 + tile_tokens, w.length) - 1) / kKeys : -1;
+    }
+    if (n >= 2) ok = await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait);
+    if (!ok) break;
+    if (lane == 0) {
+      sm.item[slot] = w;
+      mbar_arrive(&sm.item_full[slot]);
+    }
+    __syncwarp();
+    if (!more) break;
+    const int last_any = max(w.last[0], w.last[1]);
+    if (lane == 0) {
+#pragma unroll
+      for (int t = 0; t < kQTiles; ++t)
+        if (ok && w.last[t] >= 0) {
+          if (q_used[t] > 0) ok = await(&sm.q_empty[t], (uint32_t)(q_used[t] - 1) & 1u, &sm.wait);
+          if (ok)
+            tma_load_tile<kTile>(sm.q[t], &p.q_map, head * p.group, w.row0 + w.tok0 + t * tile_tokens, &sm.q_full[t]);
+          ++q_used[t];
+        }
+      for (int j = 0; ok && j <= last_any; ++j, ++tiles) {
+        const int stage = tiles % kStages, use = tiles / kStages, row = w.row0 + j * kKeys;
+        if (use > 0) ok = await(&sm.k_empty[stage], (uint32_t)(use - 1) & 1u, &sm.wait);
+        if (ok && j != p.skip_tile) tma_load_tile<kKeys>(sm.k[stage], &p.k_map, head, row, &sm.k_full[stage]);
+        if (ok && use > 0) ok = await(&sm.v_empty[stage], (uint32_t)(use - 1) & 1u, &sm.wait);
+        if (ok) tma_load_tile<kKeys>(sm.v[stage], &p.v_map, head, row, &sm.v_full[stage]);
       }
-      return;
     }
-    left -= __shfl_sync(0xffffffffu, upto, 31);
+    ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    if (!ok) break;
   }
-  if (lane == 0) sm.tile = -1;
-}
-
-__device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& sm, const PromptWork& w) {
-  mbar_expect_tx(&sm.q_full, kQTiles * kTileBytes);
-#pragma unroll
-  for (int t = 0; t < kQTiles; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      tma_load(sm.q[t] + h * kHalfTile, &p.q_map, 64 * h, w.head * p.group, w.row0 + w.tok0 + t * w.tile_tokens, &sm.q_full);
-  int loaded = 0;
-  for (; loaded <= w.last_any; ++loaded) {
-    const int stage = loaded % kStages, use = loaded / kStages, row = w.row0 + loaded * kTile;
-    if (use > 0 && !bounded_wait(&sm.k_empty[stage], (use - 1) & 1u, &sm.wait)) break;
-    if (loaded != p.skip_tile) {
-      mbar_expect_tx(&sm.k_full[stage], kTileBytes);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        tma_load(sm.k[stage] + h * kHalfTile, &p.k_map, 64 * h, w.head, row, &sm.k_full[stage]);
-    }
-    if (use > 0 && !bounded_wait(&sm.v_empty[stage], (use - 1) & 1u, &sm.wait)) break;
-    mbar_expect_tx(&sm.v_full[stage], kTileBytes);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      tma_load(sm.v[stage] + h * kHalfTile, &p.v_map, 64 * h, w.head, row, &sm.v_full[stage]);
-  }
-  if (!*(volatile int*)&sm.wait.abort) return;
-  // A wait ran out somewhere: shared memory is given back at the end of the
-  // kernel, so this thread stays until its own copies have landed.
-  for (int tile = max(0, loaded - kStages); tile <= min(loaded, w.last_any); ++tile) {
-    const int stage = tile % kStages;
-    const uint32_t parity = (uint32_t)(tile / kStages) & 1u;
-    for (int tries = 0; tries < 1000 && tile != p.skip_tile && !mbar_try(&sm.k_full[stage], parity, 1000u); ++tries) {
-    }
-    for (int tries = 0; tries < 1000 && tile < loaded && !mbar_try(&sm.v_full[stage], parity, 1000u); ++tries) {
-    }
+  if (lane != 0 || !*(volatile int*)&sm.wait.abort) return;
+  // A wait ran out somewhere.  Shared memory is given back at the end of the
+  // kernel, so this thread stays until its own copies have landed (bounded: a
+  // tile that was left out never lands).
+  for (int b = 0; b < 2 * kStages + kQTiles; ++b) {
+    uint64_t* bar = b < kStages ? &sm.k_full[b] : b < 2 * kStages ? &sm.v_full[b - kStages] : &sm.q_full[b - 2 * kStages];
+    for (int parity = 0; parity < 2; ++parity)
+      for (int tries = 0; tries < 100 && !mbar_try(bar, (uint32_t)parity, 1000u); ++tries) {
+      }
   }
 }
 
-// Rows (tokens) valid .. 127 of a V tile become zero: they belong to another
-// prompt or to nothing, and whatever they hold must not meet a zero probability.
+// Rows (tokens) valid .. of a V tile become zero: they belong to another prompt
+// or to nothing, and whatever they hold must not meet a zero probability.
 __device__ __forceinline__ void clear_value_rows(uint8_t* tile, int valid, int lane) {
-  for (int x = valid * 16 + lane; x < kTile * 16; x += 32) {
+  for (int x = valid * 16 + lane; x < kKeys * 16; x += 32) {
     const int row = x >> 4, chunk = x & 15;
-    *reinterpret_cast<uint4*>(tile + (chunk >> 3) * kHalfTile + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4*>(tile + (chunk >> 3) * kKeyHalf + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// The warp that issues the products: S_t(0); then per key tile j and query tile
-// t: O_t(j), S_t(j + 1).
-__device__ __forceinline__ void prompt_issue(PromptSmem& sm, const PromptWork& w, uint32_t tmem, int lane) {
-  const auto after_wait = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
-  const auto scores = [&](int t, int j) {
-    if (lane == 0) {
-      tile_product(tmem + (uint32_t)(t * kTile), smem_addr(sm.q[t]), smem_addr(sm.k[j % kStages]), false);
-      umma_commit(&sm.s_ready[t]);
-    }
-  };
-  const auto last_tile = [&](int j) { return j <= w.last[kQTiles - 1] ? kQTiles - 1 : 0; };
-  bounded_wait(&sm.q_full, 0u, &sm.wait);
-  bounded_wait(&sm.k_full[0], 0u, &sm.wait);
-  after_wait();
-#pragma unroll
-  for (int t = 0; t < kQTiles; ++t)
-    if (w.last[t] >= 0) scores(t, 0);
-  if (lane == 0) umma_commit(&sm.k_empty[0]);
-  for (int j = 0; j <= w.last_any; ++j) {
-    const int stage = j % kStages, next = (j + 1) % kStages;
-    const uint32_t parity = (uint32_t)(j / kStages) & 1u, next_parity = (uint32_t)((j + 1) / kStages) & 1u;
-    bool v_seen = false, k_seen = false;
-#pragma unroll
-    for (int t = 0; t < kQTiles; ++t) {
-      if (j <= w.last[t]) {
-        if (!v_seen) {
-          bounded_wait(&sm.v_full[stage], parity, &sm.wait);
-          const int valid = w.length - j * kTile;
-          if (valid < kTile) clear_value_rows(sm.v[stage], valid, lane);
-          __syncwarp();
-        }
-        v_seen = true;
-        bounded_wait(&sm.p_ready[t], (uint32_t)j & 1u, &sm.wait);
-        after_wait();
-        if (lane == 0) {
-          // P_t sits in the first half of S_t's columns.
-          value_product(tmem + (uint32_t)((kQTiles + t) * kTile), tmem + (uint32_t)(t * kTile),
-                        smem_addr(sm.v[stage]), j > 0);
-          umma_commit(&sm.o_done[t]);
-          if (t == last_tile(j)) umma_commit(&sm.v_empty[stage]);
-        }
-      }
-      if (j + 1 <= w.last[t]) {
-        if (!k_seen) bounded_wait(&sm.k_full[next], next_parity, &sm.wait);
-        k_seen = true;
-        after_wait();
-        scores(t, j + 1);
-        if (lane == 0 && t == last_tile(j + 1)) umma_commit(&sm.k_empty[next]);
-      }
-      __syncwarp();
-    }
-  }
-  // Nothing may still be running when tensor memory is given back, also when a
-  // wait above gave up and the roles ran ahead.
-  if (lane == 0) {
-    umma_commit(&sm.drained);
+// Nothing that this warp issued may still be running when tensor memory is given
+// back, also when a wait gave up and the roles ran ahead.
+__device__ __forceinline__ void drain(uint64_t* bar) {
+  __syncwarp();
+  commit(bar);
 #pragma unroll 1
-    for (int tries = 0; tries < (1 << 20); ++tries)
-      if (mbar_try(&sm.drained, 0u, 1000u)) break;
-  }
+  for (int tries = 0; tries < (1 << 20); ++tries)
+    if (mbar_try(bar, 0u, 1000u)) break;
   __syncwarp();
 }
 
-template <bool kMasked>
-__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], int first, int visible, float m) {
-#pragma unroll
-  for (int x = 0; x < 32; ++x)
-    if (!kMasked || first + x <= visible) m = fmaxf(m, __uint_as_float(s[x]));
-  return m;
+// Takes the next item; false: none is left (or a wait ran out).
+__device__ __forceinline__ bool next_item(PromptSmem& sm, int n, int lane, Item& w) {
+  const int slot = n & 1;
+  if (!await(&sm.item_full[slot], (uint32_t)(n >> 1) & 1u, &sm.wait)) return false;
+  w = sm.item[slot];
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
+  return w.head >= 0;
 }
 
-// exp2(score * scale - ref) of 32 scores as 16 BF16 pairs; returns their sum
-// (of the unrounded values).
-template <bool kMasked>
-__device__ __forceinline__ float chunk_probabilities(const uint32_t (&s)[32], int first, int visible, float scale,
-                                                     float ref, uint32_t (&packed)[16]) {
-  float sum = 0.f;
+// The warp that issues the score products, key tile by key tile for both query
+// tiles: S_t(j) as soon as the softmax has taken S_t(j - 1).
+__device__ __forceinline__ void issue_scores(PromptSmem& sm, uint32_t tmem, int lane) {
+  uint32_t items[kQTiles] = {0, 0}, issued[kQTiles] = {0, 0};
+  uint32_t tile = 0;  // key tiles so far
+  Item w;
+  for (int n = 0; next_item(sm, n, lane, w); ++n) {
+    const int last_any = max(w.last[0], w.last[1]);
+#pragma unroll 1
+    for (int j = 0; j <= last_any; ++j, ++tile) {
+      const uint32_t stage = tile % kStages;
+      await(&sm.k_full[stage], (tile / kStages) & 1u, &sm.wait);
 #pragma unroll
-  for (int x = 0; x < 32; x += 2) {
-    float a = ex2(fmaf(__uint_as_float(s[x]), scale, -ref));
-    float b = ex2(fmaf(__uint_as_float(s[x + 1]), scale, -ref));
-    if (kMasked && first + x > visible) a = 0.f;
-    if (kMasked && first + x + 1 > visible) b = 0.f;
-    sum += a + b;
-    const __nv_bfloat162 pair = __floats2bfloat162_rn(a, b);
-    packed[x >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
+      for (int t = 0; t < kQTiles; ++t) {
+        if (j > w.last[t]) continue;
+        if (j == 0) await(&sm.q_full[t], items[t]++ & 1u, &sm.wait);
+        if (issued[t] > 0) await(&sm.s_free[t], (issued[t] - 1) & 1u, &sm.wait);
+        ++issued[t];
+        __syncwarp();
+        tmem_acquire();
+        score_product(tmem + kTmemS + (uint32_t)(t * kKeys), key_desc_low(smem_addr(sm.q[t])),
+                      key_desc_low(smem_addr(sm.k[stage])));
+        commit(&sm.s_ready[t]);
+        if (j == w.last[t]) commit(&sm.q_empty[t]);
+      }
+      commit(&sm.k_empty[stage]);
+    }
   }
-  return sum;
+  drain(&sm.drained[0]);
 }
+
+// The warp that issues the value products: O_t(j) as soon as P_t(j) is written.
+__device__ __forceinline__ void issue_values(PromptSmem& sm, uint32_t tmem, int lane) {
+  uint32_t items[kQTiles] = {0, 0}, issued[kQTiles] = {0, 0};
+  uint32_t tile = 0;  // key tiles so far
+  Item w;
+  for (int n = 0; next_item(sm, n, lane, w); ++n) {
+    const int last_any = max(w.last[0], w.last[1]);
+#pragma unroll 1
+    for (int j = 0; j <= last_any; ++j, ++tile) {
+      const uint32_t stage = tile % kStages;
+      await(&sm.v_full[stage], (tile / kStages) & 1u, &sm.wait);
+      const int valid = w.length - j * kKeys;
+      if (valid < kKeys) clear_value_rows(sm.v[stage], valid, lane);
+#pragma unroll
+      for (int t = 0; t < kQTiles; ++t) {
+        if (j > w.last[t]) continue;
+        // The result warps have read the item before's O.
+        if (j == 0 && items[t]++ > 0) await(&sm.o_free[t], items[t] & 1u, &sm.wait);
+        await(&sm.p_ready[t], issued[t]++ & 1u, &sm.wait);
+        __syncwarp();
+        tmem_acquire();
+        value_product(tmem + (uint32_t)(t * kTile), tmem + kTmemP + (uint32_t)(t * kKeys / 2),
+                      value_desc_low(smem_addr(sm.v[stage])), j > 0);
+        commit(&sm.p_free[t]);
+        if (j == w.last[t]) commit(&sm.o_done[t]);
+      }
+      commit(&sm.v_empty[stage]);
+    }
+  }
+  drain(&sm.drained[1]);
+}
+
+// ---------------------------------------------------------------------------
+// Softmax.
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float low, float high) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  return r;
+}
+
+// 2^x of two values of at most about 8 on the FP32 pipe: x = n + f with n the
+// nearest integer (added and taken off again at 1.5 * 2^23, whose low bits then
+// hold n), 2^f by a polynomial that is exact at 0, n added to the exponent.
+// Below -127 the result is 0.  The coefficients are a least-maximum fit of the
+// relative error over [-1/2, 1/2]: 1.0e-4, a 39th of the half step of BF16.
+constexpr float kExp1 = 0.69328290f, kExp2 = 0.24221097f, kExp3 = 0.05500906f;
+__device__ __forceinline__ uint64_t exp2_polynomial(uint64_t x) {
+  float a, b;
+  unpack2(x, a, b);
+  x = pack2(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const uint64_t big = pack2(12582912.f, 12582912.f), minus_big = pack2(-12582912.f, -12582912.f);
+  const uint64_t shifted = add2(x, big);
+  const uint64_t whole = add2(shifted, minus_big);
+  const uint64_t f = fma2(whole, pack2(-1.f, -1.f), x);
+  uint64_t y = fma2(f, pack2(kExp3, kExp3), pack2(kExp2, kExp2));
+  y = fma2(f, y, pack2(kExp1, kExp1));
+  y = fma2(f, y, pack2(1.f, 1.f));
+  float na, nb;
+  unpack2(shifted, na, nb);
+  unpack2(y, a, b);
+  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23)),
+               __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23)));
+}
+
+// Loads or stores kCount 32-bit columns of this thread's lane, in pieces of 32,
+// 16 and 8; the caller waits.
+template <int kCount>
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t* r) {
+  if constexpr (kCount >= 32) {
+    tmem_load32_async(at, *reinterpret_cast<uint32_t(*)[32]>(r));
+    tmem_load<kCount - 32>(at + 32, r + 32);
+  } else if constexpr (kCount >= 16) {
+    tmem_load16_async(at, *reinterpret_cast<uint32_t(*)[16]>(r));
+    tmem_load<kCount - 16>(at + 16, r + 16);
+  } else {
+    static_assert(kCount == 0, "columns come in sixteens");
+  }
+}
+template <int kCount>
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t* r) {
+  if constexpr (kCount >= 16) {
+    tmem_store16(at, *reinterpret_cast<const uint32_t(*)[16]>(r));
+    tmem_store<kCount - 16>(at + 16, r + 16);
+  } else if constexpr (kCount >= 8) {
+    tmem_store8(at, *reinterpret_cast<const uint32_t(*)[8]>(r));
+    tmem_store<kCount - 8>(at + 8, r + 8);
+  } else {
+    static_assert(kCount == 0, "columns come in eights");
+  }
+}
+
+// Softmax warps of query tile `mine`: a thread has one query row and, of the
+// tile's columns, part `part` of kParts.
+__device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int mine, int part,
+                                               int row) {
+  constexpr int kCols = kKeys / kParts, kOCols = kTile / kParts;
+  const int lane = row & 31, rows = row >> 5;
+  const uint32_t lanes = (uint32_t)(32 * rows) << 16;
+  const uint32_t tmem_s = tmem + lanes + kTmemS + (uint32_t)(mine * kKeys + part * kCols);
+  const uint32_t tmem_p = tmem + lanes + kTmemP + (uint32_t)(mine * (kKeys / 2) + part * (kCols / 2));
+  const uint32_t tmem_o = tmem + lanes + (uint32_t)(mine * kTile + part * kOCols);
+  const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+  uint32_t s_used = 0, sums = 0, met = 0;
+  // What the other thread of the row has.
+  const auto exchange = [&](float x) {
+    float* at = sm.half_row[met & 1][mine][0] + row;
+    ++met;
+    at[part * kTile] = x;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * mine + rows) : "memory");
+    return at[(part ^ 1) * kTile];
+  };
+  // Whether any thread of these rows asks for it.
+  const auto any_row = [&](bool asks) -> bool {
+    if constexpr (kParts == 1) return __any_sync(0xffffffffu, asks);
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred q, r;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.or.pred r, %2, 64, q;\n\tselp.b32 %0, 1, 0, r;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)asks), "r"(1 + 4 * mine + rows)
+        : "memory");
+    return any != 0;
+  };
+  Item w;
+  for (int n = 0; next_item(sm, n, lane, w); ++n) {
+    const int my_last = w.last[mine];
+    // Rows past the prompt compute like its last token.
+    const int position = min(w.tok0 + (mine * kTile + row) / p.group, w.length - 1) - part * kCols;
+    // Key tiles below this one are seen whole by every row.
+    const int first_masked = (w.tok0 + mine * kTile / p.group + 1) / kKeys;
+    float ref = 0.f;  // reference point of the exponentials
+    uint64_t row_sum[2] = {0, 0};
+    const auto step = [&](int j, auto masked) {
+      await(&sm.s_ready[mine], s_used & 1u, &sm.wait);
+      ++s_used;
+      tmem_acquire();
+      uint32_t s[kCols];
+      tmem_load<kCols>(tmem_s, s);
+      tmem_wait_loads();
+      tmem_release();
+      mbar_arrive(&sm.s_free[mine]);
+      if constexpr (decltype(masked)::value) {
+        const int visible = position - j * kKeys;  // columns 0..visible of this part count
+#pragma unroll
+        for (int x = 0; x < kCols; ++x)
+          if (x > visible) s[x] = 0xff800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int x = 0; x < kCols; x += 2)
+        top[(x >> 1) & 3] = max3(top[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+      // The scale is positive, so the largest raw score gives the largest scaled one.
+      float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
+      // The reference follows the running maximum once that is kRescaleSlack above it.
+      if (any_row(j == 0 || !(tile_max <= ref + kRescaleSlack))) {
+        if constexpr (kParts == 2) tile_max = max3(tile_max, exchange(tile_max), tile_max);
+        // An infinite or NaN maximum makes the whole row NaN (its output is then
+        // computed again, key by key).
+        if (!(tile_max < INFINITY)) tile_max = NAN;
+        if (j == 0) {
+          ref = tile_max == -INFINITY ? 0.f : tile_max;
+        } else {
+          float keep = 1.f;
+          if (!(tile_max <= ref + kRescaleSlack)) {
+            keep = ex2(ref - tile_max);
+            ref = tile_max;
+            row_sum[0] = fma2(row_sum[0], pack2(keep, keep), 0);
+            row_sum[1] = fma2(row_sum[1], pack2(keep, keep), 0);
+          }
+          await(&sm.p_free[mine], s_used & 1u, &sm.wait);  // the O product before this one is done
+          tmem_acquire();
+#pragma unroll 1
+          for (int c = 0; c < kOCols; c += 16) {
+            uint32_t o[16];
+            tmem_load16_async(tmem_o + (uint32_t)c, o);
+            tmem_wait_loads();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+            tmem_store16(tmem_o + (uint32_t)c, o);
+          }
+        }
+      }
+      const uint64_t minus_ref = pack2(-ref, -ref);
+      uint32_t packed[kCols / 2];
+#pragma unroll
+      for (int i = 0; i < kCols / 2; ++i) {  // pairs of columns
+        uint64_t x = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, minus_ref);
+        float a, b;
+        // A quarter of the pairs on the FP32 pipe: the special-function unit alone
+        // would take as long as both products.
+        if (i % 4 == 1) {
+          x = exp2_polynomial(x);
+          unpack2(x, a, b);
+        } else {
+          unpack2(x, a, b);
+          a = ex2(a);
+          b = ex2(b);
+          x = pack2(a, b);
+        }
+        row_sum[i & 1] = add2(row_sum[i & 1], x);
+        packed[i] = bf16_pair(a, b);
+      }
+      if (s_used > 1) await(&sm.p_free[mine], s_used & 1u, &sm.wait);
+      tmem_acquire();
+      tmem_store<kCols / 2>(tmem_p, packed);
+      tmem_wait_stores();
+      tmem_release();
+      mbar_arrive(&sm.p_ready[mine]);
+    };
+    int j = 0;
+#pragma unroll 1
+    for (; j < min(first_masked, my_last + 1); ++j) step(j, std::false_type{});
+#pragma unroll 1
+    for (; j <= my_last; ++j) step(j, std::true_type{});
+    if (my_last < 0) continue;
+    float a, b;
+    unpack2(add2(row_sum[0], row_sum[1]), a, b);
+    a += b;
+    if constexpr (kParts == 2) a += exchange(a);
+    if (part == 0) {
+      if (sums > 0) await(&sm.sum_empty[mine], (sums - 1) & 1u, &sm.wait);
+      ++sums;
+      sm.sum[mine][row] = a;
+      mbar_arrive(&sm.sum_full[mine]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Results.
 
 // One query row by one warp, key by key over the keys that it sees, lane l
 // carrying dims 4 l .. 4 l + 3.  The tensor cores also multiply the values of
 // later tokens (by zero probabilities), so a row that came out NaN or infinite
 // is computed again here: what it then shows is its own.
-__device__ __noinline__ void prompt_row(const PromptParams& p, int row0, int tok, int kv_head, int q_head, int lane) {
+__device__ __forceinline__ void prompt_row(const PromptParams& p, int row0, int tok, int kv_head, int q_head, int lane) {
   const auto load = [&](const Heads& h, int row, int head, float (&x)[4]) {
     const uint2 two = *reinterpret_cast<const uint2*>(h.at + row * h.token + head * h.head + 4 * lane);
     x[0] = __uint_as_float(two.x << 16);
@@ -286,6 +677,7 @@ __device__ __noinline__ void prompt_row(const PromptParams& p, int row0, int tok
   };
   float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
   load(p.q, row0 + tok, q_head, q);
+#pragma unroll 1
   for (int j = 0; j <= tok; ++j) {
     load(p.k, row0 + j, kv_head, k);
     load(p.v, row0 + j, kv_head, v);
@@ -304,96 +696,57 @@ __device__ __noinline__ void prompt_row(const PromptParams& p, int row0, int tok
     top = new_top;
   }
   const float inv = sum > 0.f ? 1.f / sum : sum;
-  const __nv_bfloat162 a = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), b = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
   *reinterpret_cast<uint2*>(p.out + (row0 + tok) * p.o_token + q_head * p.o_head + 4 * lane) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      make_uint2(bf16_pair(o[0] * inv, o[1] * inv), bf16_pair(o[2] * inv, o[3] * inv));
 }
 
-// Softmax warpgroup of query tile `mine`: thread = query row.
-__device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem& sm, const PromptWork& w,
-                                               uint32_t tmem, int mine, int row, int warp) {
-  const int my_last = w.last[mine];
-  if (my_last < 0) return;
-  const int tok = w.tok0 + mine * w.tile_tokens + row / p.group;
-  const int position = min(tok, w.length - 1);  // rows past the prompt compute like its last token
-  float row_max = -INFINITY, row_sum = 0.f;
-  const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;  // this warp's tensor-memory lanes
-  const uint32_t tmem_s = tmem + (uint32_t)(mine * kTile) + lane_base;
-  const uint32_t tmem_o = tmem + (uint32_t)((kQTiles + mine) * kTile) + lane_base;
-  uint32_t s[32];
-  for (int j = 0; j <= my_last; ++j) {
-    const uint32_t parity = (uint32_t)j & 1u;
-    bounded_wait(&sm.s_ready[mine], parity, &sm.wait);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const int visible = position - j * kTile;  // columns 0..visible of this tile count
-    const bool masked = __any_sync(0xffffffffu, visible < kTile - 1);
-    float raw_max = -INFINITY;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      tmem_load32(tmem_s + (uint32_t)(32 * c), s);
-      raw_max = masked ? chunk_max<true>(s, 32 * c, visible, raw_max) : chunk_max<false>(s, 32 * c, visible, raw_max);
-    }
-    const float new_max = fmaxf(row_max, raw_max * p.scale_log2);  // the scale is positive
-    const float ref = new_max == -INFINITY ? 0.f : new_max;
-    const bool rise = new_max > row_max;
-    const float keep = rise ? ex2(row_max - ref) : 1.f;
-    if (j > 0) {
-      bounded_wait(&sm.o_done[mine], parity ^ 1u, &sm.wait);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          tmem_load32(tmem_o + (uint32_t)(32 * c), s);
+// Result warps: thread = query row of both tiles.
+__device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int row) {
+  const int lane = row & 31;
+  const uint32_t tmem_o = tmem + ((uint32_t)(row & ~31) << 16);
+  uint32_t used[kQTiles] = {0, 0};
+  Item w;
+  for (int n = 0; next_item(sm, n, lane, w); ++n) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) s[x] = __float_as_uint(__uint_as_float(s[x]) * keep);
-          tmem_store32(tmem_o + (uint32_t)(32 * c), s);
+    for (int t = 0; t < kQTiles; ++t) {
+      if (w.last[t] < 0) continue;
+      await(&sm.sum_full[t], used[t] & 1u, &sm.wait);
+      const float sum = sm.sum[t][row];
+      mbar_arrive(&sm.sum_empty[t]);
+      await(&sm.o_done[t], used[t] & 1u, &sm.wait);
+      ++used[t];
+      tmem_acquire();
+      const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays NaN
+      const int of_pair = t * kTile + row, tok = w.tok0 + of_pair / p.group, g = of_pair % p.group;
+      __nv_bfloat16* dst = p.out + (int64_t)(w.row0 + tok) * p.o_token + (int64_t)(w.head * p.group + g) * p.o_head;
+      bool finite = true;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t o[32];
+        tmem_load32(tmem_o + (uint32_t)(t * kTile + c), o);
+        if (tok < w.length) {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            uint32_t packed[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float a = __uint_as_float(o[8 * ch + 2 * x]) * inv, b = __uint_as_float(o[8 * ch + 2 * x + 1]) * inv;
+              finite &= fabsf(a) < INFINITY && fabsf(b) < INFINITY;
+              packed[x] = bf16_pair(a, b);
+            }
+            *reinterpret_cast<uint4*>(dst + c + 8 * ch) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          }
         }
       }
-    }
-    row_sum *= keep;
-    row_max = new_max;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      tmem_load32(tmem_s + (uint32_t)(32 * c), s);
-      uint32_t packed[16];
-      row_sum += masked ? chunk_probabilities<true>(s, 32 * c, visible, p.scale_log2, ref, packed)
-                        : chunk_probabilities<false>(s, 32 * c, visible, p.scale_log2, ref, packed);
-      tmem_store16(tmem_s + (uint32_t)(16 * c), packed);  // over scores already read
-    }
-    tmem_wait_stores();
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    mbar_arrive(&sm.p_ready[mine]);
-  }
-
-  bounded_wait(&sm.o_done[mine], (uint32_t)my_last & 1u, &sm.wait);
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const float inv = row_sum > 0.f ? 1.f / row_sum : row_sum;  // NaN stays NaN
-  __nv_bfloat16* dst = p.out + (int64_t)(w.row0 + tok) * p.o_token + (int64_t)(w.head * p.group + row % p.group) * p.o_head;
-  bool finite = true;
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    tmem_load32(tmem_o + (uint32_t)(32 * c), s);
-    if (tok < w.length) {
-#pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        uint32_t o[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float a = __uint_as_float(s[8 * ch + 2 * x]) * inv, b = __uint_as_float(s[8 * ch + 2 * x + 1]) * inv;
-          finite &= fabsf(a) < INFINITY && fabsf(b) < INFINITY;
-          const __nv_bfloat162 pair = __floats2bfloat162_rn(a, b);
-          o[x] = *reinterpret_cast<const uint32_t*>(&pair);
-        }
-        *reinterpret_cast<uint4*>(dst + 32 * c + 8 * ch) = make_uint4(o[0], o[1], o[2], o[3]);
+      tmem_release();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_free[t]);
+      for (uint32_t again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
+        const int r = t * kTile + row - lane + __ffs(again) - 1;
+        prompt_row(p, w.row0, w.tok0 + r / p.group, w.head, w.head * p.group + r % p.group, lane);
       }
     }
   }
-  __syncwarp();
-  for (uint32_t again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
-    const int r = row - (row & 31) + __ffs(again) - 1;
-    prompt_row(p, w.row0, w.tok0 + mine * w.tile_tokens + r / p.group, w.head, w.head * p.group + r % p.group, row & 31);
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __grid_constant__ PromptParams p) {
@@ -402,25 +755,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
   extern __shared__ uint8_t dyn[];
   PromptSmem& sm = *reinterpret_cast<PromptSmem*>(dyn + ((1024u - (smem_addr(dyn) & 1023u)) & 1023u));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 0) find_work(p, sm, lane);
-  __syncthreads();
-  PromptWork w;
-  if (sm.tile < 0) return;
-  w.head = blockIdx.y;
-  w.row0 = sm.row0;
-  w.length = sm.length;
-  w.tile_tokens = kTile / p.group;
-  w.tok0 = sm.tile * kQTiles * w.tile_tokens;
-#pragma unroll
-  for (int t = 0; t < kQTiles; ++t) {
-    const int t0 = w.tok0 + t * w.tile_tokens;
-    w.last[t] = t0 < w.length ? (min(t0 + w.tile_tokens, w.length) - 1) >> 7 : -1;
-  }
-  w.last_any = max(w.last[0], w.last[kQTiles - 1]);
-
   if (tid == 0) {
-    mbar_init(&sm.q_full, 1);
-    mbar_init(&sm.drained, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.item_full[i], 1);
+      mbar_init(&sm.item_empty[i], kItemReaders);
+    }
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.k_full[i], 1);
@@ -430,10 +770,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     }
 #pragma unroll
     for (int t = 0; t < kQTiles; ++t) {
+      mbar_init(&sm.q_full[t], 1);
+      mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_ready[t], 1);
+      mbar_init(&sm.s_free[t], kParts * kTile);
+      mbar_init(&sm.p_ready[t], kParts * kTile);
+      mbar_init(&sm.p_free[t], 1);
+      mbar_init(&sm.sum_full[t], kTile);
+      mbar_init(&sm.sum_empty[t], kTile);
       mbar_init(&sm.o_done[t], 1);
-      mbar_init(&sm.p_ready[t], kTile);
+      mbar_init(&sm.o_free[t], 4);  // result warps
     }
+    mbar_init(&sm.drained[0], 1);
+    mbar_init(&sm.drained[1], 1);
     sm.wait.abort = 0;
     sm.wait.status = &g_prompt_status;
     sm.wait.limit = p.wait_limit;
@@ -447,22 +796,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  tmem_release();
   __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  tmem_acquire();
   const uint32_t tmem = sm.tmem_base;
 
-  if (tid < kSoftmaxThreads) {
-    prompt_softmax(p, sm, w, tmem, tid / kTile, tid & (kTile - 1), warp);
-  } else if (warp == kIssueWarp) {
-    prompt_issue(sm, w, tmem, lane);
-  } else if (warp == kLoadWarp && lane == 0) {
-    prompt_load(p, sm, w);
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    prompt_softmax(p, sm, tmem, warp / (4 * kParts), (warp >> 2) % kParts, tid & (kTile - 1));
+  } else if (warp < kScoreWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kResultRegs));
+    prompt_results(p, sm, tmem, tid & (kTile - 1));
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kScoreWarp) issue_scores(sm, tmem, lane);
+    if (warp == kValueWarp) issue_values(sm, tmem, lane);
+    if (warp == kLoadWarp) prompt_load(p, sm, lane);
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  tmem_release();
   __syncthreads();
   if (warp == 0) {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem_acquire();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
   }
 }
@@ -540,8 +894,8 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   PromptParams p;
   const uint32_t tile_tokens = (uint32_t)(kTile / group);
   if (int rc = head_map(p.q_map, "q", q, tokens, q_heads, q_token, q_head, (uint32_t)group, tile_tokens)) return rc;
-  if (int rc = head_map(p.k_map, "k", k, tokens, kv_heads, k_token, k_head, 1, kTile)) return rc;
-  if (int rc = head_map(p.v_map, "v", v, tokens, kv_heads, v_token, v_head, 1, kTile)) return rc;
+  if (int rc = head_map(p.k_map, "k", k, tokens, kv_heads, k_token, k_head, 1, kKeys)) return rc;
+  if (int rc = head_map(p.v_map, "v", v, tokens, kv_heads, v_token, v_head, 1, kKeys)) return rc;
   static std::atomic<uint64_t> smem_allowed;
   const int smem = (int)sizeof(PromptSmem) + 1024;
   if (int rc = allow_dynamic_smem(prompt_attn_kernel, smem, smem_allowed)) return rc;
@@ -554,13 +908,14 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.starts = starts;
   p.prompts = prompts;
   p.tokens = (int)tokens;
+  p.kv_heads = kv_heads;
   p.group = group;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_limit = wait_debug().limit;
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
   // Every prompt has at most one pair of tiles that is not full.
-  const int64_t pairs = tokens / (kQTiles * tile_tokens) + prompts;
-  prompt_attn_kernel<<<dim3((unsigned)pairs, (unsigned)kv_heads), kPromptThreads, smem, (cudaStream_t)stream>>>(p);
+  const int64_t items = (tokens / (kQTiles * tile_tokens) + prompts) * kv_heads;
+  prompt_attn_kernel<<<(unsigned)std::min<int64_t>(items, device_sms()), kPromptThreads, smem, (cudaStream_t)stream>>>(p);
   FP_LAUNCH_CHECK("prompt_attn_kernel");
   return FP_OK;
 }

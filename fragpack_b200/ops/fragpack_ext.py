@@ -23,7 +23,7 @@ _DIR = Path(__file__).resolve().parent
 # one compiled with different flags); by default the in-tree library is used.
 LIBRARY = Path(os.environ.get("FRAGPACK_B200_LIBRARY") or _DIR / "libfragpack_b200.so")
 
-_HERE: "contextlib.AbstractContextManager[None]" = contextlib.nullcontext()
+_HERE = contextlib.nullcontext()
 c_i32, c_i64, c_f32, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
 
@@ -166,15 +166,19 @@ def require_cuda(tensor: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} must be a CUDA tensor: fragpack_b200.ops has no CPU fallback")
 
 
-def on_device(device: torch.device) -> "contextlib.AbstractContextManager[None]":
-    """Make ``device`` current for a launch, if it is not already."""
-    if device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def on_device(device: int) -> contextlib.AbstractContextManager:
+    """Make CUDA device ``device`` current for a launch, if it is not already."""
+    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+# Without the Stream object (3 us of host time a call) where torch has such a getter.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr() -> int:
     """Handle of the current CUDA stream."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

@@ -53,29 +53,32 @@ def prompt_attention(
         One kernel on the current CUDA stream; CUDA-graph safe; allocates nothing.
     """
     require_cuda(q, "q")
-    if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0:
+    q_shape, kv_shape, device = q.shape, k.shape, q.get_device()
+    if len(q_shape) != 3 or len(kv_shape) != 3 or kv_shape[1] == 0:
         raise RuntimeError("q, k and v must be [T, heads, 128]")
-    tokens, kv_heads = k.shape[0], k.shape[1]
-    group = q.shape[1] // kv_heads
-    if group == 0 or group * kv_heads != q.shape[1] or GQA % group:
-        raise ValueError(f"query heads {q.shape[1]} need a group dividing {GQA}")
-    if k.shape != (tokens, kv_heads, 128) or v.shape != k.shape or q.shape[0] != tokens or q.shape[2] != 128:
+    tokens, kv_heads = kv_shape[0], kv_shape[1]
+    group = q_shape[1] // kv_heads
+    if group == 0 or group * kv_heads != q_shape[1] or GQA % group:
+        raise ValueError(f"query heads {q_shape[1]} need a group dividing {GQA}")
+    if kv_shape[2] != 128 or v.shape != kv_shape or q_shape[0] != tokens or q_shape[2] != 128:
         raise RuntimeError("q must be [T, H * G, 128] and k, v [T, H, 128]")
-    if out.shape != q.shape:
+    if out.shape != q_shape:
         raise RuntimeError("out must have the shape of q")
+    rows = []
     for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        if t.dtype != torch.bfloat16 or t.device != q.device or t.stride(2) != 1:
-            raise RuntimeError(f"{name} must be bfloat16 on {q.device} with a contiguous head dim")
+        stride = t.stride()
+        if t.dtype != torch.bfloat16 or t.get_device() != device or stride[2] != 1:
+            raise RuntimeError(f"{name} must be bfloat16 on cuda:{device} with a contiguous head dim")
+        rows.append((t.data_ptr(), stride[0], stride[1]))
     if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() == 0 or not starts.is_contiguous():
         raise RuntimeError("starts must be contiguous int32 [R + 1]")
-    if starts.device != q.device:
-        raise RuntimeError(f"starts must be on {q.device}")
-    with on_device(q.device):
+    if starts.get_device() != device:
+        raise RuntimeError(f"starts must be on cuda:{device}")
+    with on_device(device):
         check(
             extension().fp_prompt_attention(
-                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                v.stride(0), v.stride(1), starts.data_ptr(), starts.numel() - 1, tokens, out.data_ptr(),
-                out.stride(0), out.stride(1), kv_heads, group, float(scale), stream_ptr(),
+                *rows[0], *rows[1], *rows[2], starts.data_ptr(), starts.numel() - 1, tokens, *rows[3], kv_heads,
+                group, float(scale), stream_ptr(),
             )
         )
 

@@ -163,22 +163,23 @@ def make_rotary(
     return Rotary(turns, rot_dim, bool(interleaved), factor, native)
 
 
-def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: torch.device) -> FpHeads:
-    """Check one set of heads and its result and describe them to the library."""
-    if heads.dim() != 3 or heads.shape[2] != HEAD_DIM or heads.stride(2) != 1:
+def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: int) -> FpHeads:
+    """Check one set of heads and its result on CUDA device ``device`` and describe them to the library."""
+    shape, stride = heads.shape, heads.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
         raise RuntimeError(f"{name} must be [T, heads, {HEAD_DIM}] with a contiguous head dim")
-    if heads.shape[0] != tokens:
-        raise RuntimeError(f"{name} has {heads.shape[0]} tokens, not {tokens}")
-    if heads.dtype != torch.bfloat16 or heads.device != device:
-        raise RuntimeError(f"{name} must be bfloat16 on {device}")
+    if shape[0] != tokens:
+        raise RuntimeError(f"{name} has {shape[0]} tokens, not {tokens}")
+    if heads.dtype != torch.bfloat16 or heads.get_device() != device:
+        raise RuntimeError(f"{name} must be bfloat16 on cuda:{device}")
     if out is None:
-        return FpHeads(heads.data_ptr(), None, heads.stride(0), heads.stride(1), 0, 0, heads.shape[1])
-    if out.shape != heads.shape or out.stride(2) != 1:
+        return FpHeads(heads.data_ptr(), None, stride[0], stride[1], 0, 0, shape[1])
+    out_stride = out.stride()
+    if out.shape != shape or out_stride[2] != 1:
         raise RuntimeError(f"{name}_out must have the shape of {name} and a contiguous head dim")
-    if out.dtype != torch.bfloat16 or out.device != device:
-        raise RuntimeError(f"{name}_out must be bfloat16 on {device}")
-    return FpHeads(heads.data_ptr(), out.data_ptr(), heads.stride(0), heads.stride(1), out.stride(0),
-                   out.stride(1), heads.shape[1])
+    if out.dtype != torch.bfloat16 or out.get_device() != device:
+        raise RuntimeError(f"{name}_out must be bfloat16 on cuda:{device}")
+    return FpHeads(heads.data_ptr(), out.data_ptr(), stride[0], stride[1], out_stride[0], out_stride[1], shape[1])
 
 
 def rotary_operands(
@@ -187,7 +188,7 @@ def rotary_operands(
     rotary: Rotary,
     query_weight: torch.Tensor | None,
     key_weight: torch.Tensor | None,
-    device: torch.device,
+    device: int,
 ) -> tuple[int | None, int | None, int, int, int]:
     """Check what :func:`norm_rotary` and ``HbmKvStore.append`` share.
 
@@ -195,26 +196,29 @@ def rotary_operands(
         Pointers of the two weights, whether they are FP32, the pointer of the
         positions and whether those are int64.
     """
-    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,):
+    wide = positions.dtype == torch.int64
+    if not wide and positions.dtype != torch.int32 or positions.dim() != 1 or positions.numel() != tokens:
         raise RuntimeError(f"positions must be int64 or int32 [{tokens}]")
-    if not positions.is_contiguous() or positions.device != device or rotary.turns.device != device:
-        raise RuntimeError(f"positions must be contiguous and on {device}, like the rotary's frequencies")
-    dtype = None
-    for weight in (query_weight, key_weight):
-        if weight is None:
-            continue
-        if weight.dtype not in (torch.bfloat16, torch.float32) or weight.dtype != (dtype or weight.dtype):
+    if not positions.is_contiguous() or positions.get_device() != device or rotary.turns.get_device() != device:
+        raise RuntimeError(f"positions must be contiguous and on cuda:{device}, like the rotary's frequencies")
+    q = k = dtype = None
+    if query_weight is not None:
+        q, dtype = _weight(query_weight, device)
+    if key_weight is not None:
+        k, other = _weight(key_weight, device)
+        if dtype not in (None, other):
             raise RuntimeError("norm weights must both be bfloat16 or both float32")
-        if weight.shape != (HEAD_DIM,) or not weight.is_contiguous() or weight.device != device:
-            raise RuntimeError(f"norm weights must be contiguous [{HEAD_DIM}] on {device}")
-        dtype = weight.dtype
-    return (
-        None if query_weight is None else query_weight.data_ptr(),
-        None if key_weight is None else key_weight.data_ptr(),
-        int(dtype == torch.float32),
-        positions.data_ptr(),
-        int(positions.dtype == torch.int64),
-    )
+        dtype = other
+    return q, k, int(dtype == torch.float32), positions.data_ptr(), int(wide)
+
+
+def _weight(weight: torch.Tensor, device: int) -> tuple[int, torch.dtype]:
+    dtype = weight.dtype
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError("norm weights must both be bfloat16 or both float32")
+    if weight.dim() != 1 or weight.numel() != HEAD_DIM or not weight.is_contiguous() or weight.get_device() != device:
+        raise RuntimeError(f"norm weights must be contiguous [{HEAD_DIM}] on cuda:{device}")
+    return weight.data_ptr(), dtype
 
 
 _NO_HEADS = FpHeads(None, None, 0, 0, 0, 0, 0)
@@ -257,7 +261,7 @@ def norm_rotary(
     require_cuda(query, "query")
     if (key is None) != (key_out is None):
         raise RuntimeError("key and key_out come together")
-    device, tokens = query.device, query.shape[0]
+    device, tokens = query.get_device(), query.shape[0]
     q = head_set("query", query, query_out, tokens, device)
     k = _NO_HEADS if key is None else head_set("key", key, key_out, tokens, device)
     operands = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
