@@ -30,12 +30,12 @@
 //   result warps   divide an item's O by the sums and store it
 //   score warp     issues S products, value warp O products (one elected lane;
 //                  two warps, so that neither waits behind the other's barriers)
-//   load warp      picks the CTA's items and loads their tiles
+//   load warp      loads the items' tiles
+//   item warp      picks the CTA's items, up to two ahead of the others
 #include <cuda.h>
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "fp_api.h"
 #include "fp_common.cuh"
@@ -47,21 +47,20 @@ namespace {
 
 constexpr int kQTiles = 2;
 constexpr int kKeys = 80;                  // keys of a tile
-constexpr int kParts = 1;                  // softmax threads of a query row
 constexpr int kStages = 3;                 // K tiles and V tiles in flight, each
 constexpr int kKeyTileBytes = kKeys * 256;
 constexpr int kKeyHalf = kKeys * 128;      // one 64-dim half of a K or V tile
-constexpr int kSoftmaxWarps = 8 * kParts, kResultWarps = 4;
-constexpr int kScoreWarp = kSoftmaxWarps + kResultWarps, kValueWarp = kScoreWarp + 1, kLoadWarp = kScoreWarp + 2;
+constexpr int kSoftmaxWarps = 8, kResultWarps = 4;
+constexpr int kScoreWarp = kSoftmaxWarps + kResultWarps, kValueWarp = kScoreWarp + 1, kLoadWarp = kScoreWarp + 2,
+              kItemWarp = kScoreWarp + 3;
 constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kResultWarps + 4);  // whole warpgroups
-constexpr int kItemReaders = kValueWarp + 1;  // warps that read an item's description
+constexpr int kItemReaders = kLoadWarp + 1;  // warps that read an item's description
 // Tensor memory columns: O tiles, S tiles, P tiles.
 constexpr uint32_t kTmemColumns = 512, kTmemS = kQTiles * kTile, kTmemP = kTmemS + kQTiles * kKeys;
 static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "tensor memory is full");
-// Registers of the softmax warps, of the result warps and of the rest; together
-// what the block is launched with.
-constexpr int kSoftmaxRegs = kParts == 1 ? 184 : 96, kResultRegs = kParts == 1 ? 88 : 56,
-              kOtherRegs = kParts == 1 ? 56 : 40;
+// Registers of the softmax warps, of the result warps and of the rest: 256 x 184
+// + 128 x 88 + 128 x 56 = 512 x 128, what the block is launched with.
+constexpr int kSoftmaxRegs = 184, kResultRegs = 88, kOtherRegs = 56;
 // How far (log2 units) a row's maximum may rise above the reference point of its
 // exponentials before the reference follows and O is rescaled.
 constexpr float kRescaleSlack = 8.f;
@@ -77,16 +76,17 @@ struct Item {
 
 struct PromptSmem {
   __align__(1024) uint8_t q[kQTiles][kTileBytes];
+  __align__(1024) uint8_t o[kTileBytes];  // results on their way out
   __align__(1024) uint8_t k[kStages][kKeyTileBytes];
   __align__(1024) uint8_t v[kStages][kKeyTileBytes];
-  float sum[kQTiles][kTile];             // of the probabilities of each row
-  float half_row[2][kQTiles][2][kTile];  // what the two softmax threads of a row exchange
+  float sum[kQTiles][kTile];  // of the probabilities of each row
   Item item[2];
   __align__(8) uint64_t item_full[2], item_empty[2];
   uint64_t q_full[kQTiles], q_empty[kQTiles];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_ready[kQTiles], s_free[kQTiles];         // S product done; S read
   uint64_t p_ready[kQTiles], p_free[kQTiles];         // P written and O rescaled; O product done
+  uint64_t turn[kQTiles][4];                          // a tile's turn at the exponentials, per 32 rows
   uint64_t sum_full[kQTiles], sum_empty[kQTiles];
   uint64_t o_done[kQTiles], o_free[kQTiles];          // the item's last O product done; O read
   uint64_t drained[2];
@@ -106,7 +106,8 @@ struct PromptParams {
   __nv_bfloat16* out;
   int64_t o_token, o_head;
   const int32_t* starts;
-  int prompts, tokens, kv_heads, group;
+  int prompts, tokens, kv_heads;
+  int group, group_log2;
   float scale_log2;
   long long wait_limit;
   int skip_tile;  // test hook: this K tile of an item is not loaded (-1: none)
@@ -129,16 +130,20 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, WaitState*
   volatile int* abort = &ws->abort;
   const long long t0 = clock64();
 #pragma unroll 1
-  while (!*abort) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (arrived(bar, parity)) return true;
+  while (!arrived(bar, parity)) {
+    if (*abort) return false;
     if (clock64() - t0 > ws->limit) {
       *abort = 1;
       atomicOr(ws->status, FP_DECODE_WAIT_TIMEOUT);
     }
   }
-  return false;
+  return true;
+}
+
+// One arrival for the whole warp.
+__device__ __forceinline__ void arrive_warp(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 
 __device__ __forceinline__ void tmem_acquire() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -227,119 +232,153 @@ __device__ __forceinline__ void commit(uint64_t* bar, bool wanted = true) {
 }
 
 // ---------------------------------------------------------------------------
-// Items.  Item x of a KV head is a pair of query tiles of some prompt; pair i of
-// a prompt costs the more the larger i is, and the same in every prompt.
+// Items.  An item is a pair of query tiles of some prompt and a KV head; pair i
+// of a prompt costs the more the larger i is, and the same in every prompt.
 
-// One lane per prompt, 32 at a time: f(prompt index, first row, rows) of every
-// prompt, in order; stops when f returns true (f is warp-uniform).
-template <typename F>
-__device__ __forceinline__ void each_prompts(const PromptParams& p, int lane, F&& f) {
-#pragma unroll 1
-  for (int base = 0; base < p.prompts; base += 32) {
-    const int r = base + lane;
-    int row0 = 0, length = 0;
-    if (r < p.prompts) {
-      row0 = max(0, min(p.starts[r], p.tokens));
-      length = max(0, min(p.starts[r + 1], p.tokens) - row0);
-    }
-    if (f(row0, length)) return;
+// A prompt as a lane has it, in groups of 32: the first kKept groups stay in
+// registers, further ones are read again whenever they are asked for.
+struct Prompt {
+  int row0, length, pairs;
+};
+constexpr int kKept = 4;
+
+__device__ __forceinline__ Prompt load_prompt(const PromptParams& p, int r) {
+  Prompt x{0, 0, 0};
+  if (r < p.prompts) {
+    x.row0 = max(0, min(p.starts[r], p.tokens));
+    x.length = max(0, min(p.starts[r + 1], p.tokens) - x.row0);
   }
+  x.pairs = (x.length + (kQTiles * kTile >> p.group_log2) - 1) >> (8 - p.group_log2);
+  return x;
 }
 
-// Finds item x of the order "all prompts' pairs i, from the largest i down";
-// false: there are fewer.  The whole warp calls; every lane gets the result.
-__device__ __forceinline__ bool find_item(const PromptParams& p, int x, int lane, int& row0, int& length, int& pair) {
-  const int pair_tokens = kQTiles * kTile / p.group;
-  const auto pairs_of = [&](int rows) { return (rows + pair_tokens - 1) / pair_tokens; };
-  // Pairs with index >= level, over all prompts.
-  const auto pairs_from = [&](int level) {
-    int count = 0;
-    each_prompts(p, lane, [&](int, int rows) {
-      count += (int)__reduce_add_sync(0xffffffffu, (unsigned)max(0, pairs_of(rows) - level));
+// Picks the CTA's items, one warp.  Items come in the order "all prompts' pairs
+// i, from the largest i down" (for every KV head), so that the longest are under
+// way first, and CTAs take them forwards and backwards in turn, so that the sums
+// of what they get stay close.  The warp walks down the levels i; `above` counts
+// the pairs of the levels done.
+__device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& sm, int lane) {
+  Prompt kept[kKept];
+#pragma unroll
+  for (int g = 0; g < kKept; ++g) kept[g] = load_prompt(p, 32 * g + lane);
+  // f(group of 32 prompts) in order, until it returns true (f is warp-uniform).
+  const auto each_group = [&](auto&& f) {
+#pragma unroll
+    for (int g = 0; g < kKept; ++g) {
+      if (32 * g >= p.prompts) return;
+      if (f(kept[g])) return;
+    }
+#pragma unroll 1
+    for (int r = 32 * kKept; r < p.prompts; r += 32)
+      if (f(load_prompt(p, r + lane))) return;
+  };
+  int level = 0, above = 0, here = 0;  // `here`: prompts that have a pair of this level
+  const auto count_level = [&] {
+    here = 0;
+    each_group([&](const Prompt& x) {
+      here += __popc(__ballot_sync(0xffffffffu, x.pairs > level));
       return false;
     });
-    return count;
   };
-  if (x >= pairs_from(0)) return false;
-  int low = 0, high = (p.tokens + pair_tokens - 1) / pair_tokens;  // pairs_from(low) > x >= pairs_from(high)
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (pairs_from(mid) > x) low = mid; else high = mid;
-  }
-  pair = low;
-  int rank = x - pairs_from(low + 1);
-  each_prompts(p, lane, [&](int first, int rows) {
-    const uint32_t have = __ballot_sync(0xffffffffu, pairs_of(rows) > low);
-    const int count = __popc(have);
-    if (rank >= count) {
-      rank -= count;
-      return false;
-    }
-    const int src = __fns(have, 0, rank + 1);
-    row0 = __shfl_sync(0xffffffffu, first, src);
-    length = __shfl_sync(0xffffffffu, rows, src);
-    return true;
+  each_group([&](const Prompt& x) {
+    level = max(level, (int)__reduce_max_sync(0xffffffffu, (unsigned)x.pairs));
+    return false;
   });
-  return true;
-}
-
-__device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& sm, int lane) {
-  const int tile_tokens = kTile / p.group;
-  int q_used[kQTiles] = {0, 0};
-  int tiles = 0;  // key tiles loaded by this CTA so far
-  bool ok = true;
+  --level;
+  if (level >= 0) count_level();
+  const int tile_tokens = kTile >> p.group_log2;
   for (int n = 0;; ++n) {
     const int slot = n & 1;
-    // CTAs take items forwards and backwards in turn, so that the sums of what
-    // they get stay close.
     const int64_t at = (int64_t)n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    const int head = (int)(at % p.kv_heads);
-    Item w;
-    int pair = 0;
-    const bool more = at / p.kv_heads < (1 << 30) &&
-                      find_item(p, (int)(at / p.kv_heads), lane, w.row0, w.length, pair);
-    w.head = more ? head : -1;
-    w.tok0 = pair * kQTiles * tile_tokens;
-#pragma unroll
-    for (int t = 0; t < kQTiles; ++t) {
-      const int t0 = w.tok0 + t * tile_tokens;
-      w.last[t] = more && t0 < w.length ? (min(t0 + tile_tokens, w.length) - 1) / kKeys : -1;
+    const int64_t x = at / p.kv_heads;  // pair of every head
+    while (level >= 0 && x >= above + here) {
+      above += here;
+      if (--level >= 0) count_level();
     }
-    if (n >= 2) ok = await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait);
-    if (!ok) break;
+    Item w;
+    w.head = -1;
+    w.tok0 = max(level, 0) * kQTiles * tile_tokens;
+    w.last[0] = w.last[1] = -1;
+    if (level >= 0) {
+      w.head = (int)(at % p.kv_heads);
+      int rank = (int)(x - above);
+      each_group([&](const Prompt& of) {
+        const uint32_t have = __ballot_sync(0xffffffffu, of.pairs > level);
+        const int count = __popc(have);
+        if (rank >= count) {
+          rank -= count;
+          return false;
+        }
+        const int src = __fns(have, 0, rank + 1);
+        w.row0 = __shfl_sync(0xffffffffu, of.row0, src);
+        w.length = __shfl_sync(0xffffffffu, of.length, src);
+        return true;
+      });
+#pragma unroll
+      for (int t = 0; t < kQTiles; ++t) {
+        const int t0 = w.tok0 + t * tile_tokens;
+        if (t0 < w.length) w.last[t] = (min(t0 + tile_tokens, w.length) - 1) / kKeys;
+      }
+    }
+    if (n >= 2 && !await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) return;
     if (lane == 0) {
       sm.item[slot] = w;
       mbar_arrive(&sm.item_full[slot]);
     }
     __syncwarp();
-    if (!more) break;
+    if (w.head < 0) return;
+  }
+}
+
+// Takes the next item; false: none is left (or a wait ran out).
+__device__ __forceinline__ bool next_item(PromptSmem& sm, int n, int lane, Item& w) {
+  const int slot = n & 1;
+  if (!await(&sm.item_full[slot], (uint32_t)(n >> 1) & 1u, &sm.wait)) return false;
+  w = sm.item[slot];
+  arrive_warp(&sm.item_empty[slot], lane);
+  return w.head >= 0;
+}
+
+__device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& sm, int lane) {
+  const int tile_tokens = kTile >> p.group_log2;
+  uint32_t q_used[kQTiles] = {0, 0};
+  uint32_t tile = 0;  // key tiles so far
+  bool ok = true;
+  Item w;
+  for (int n = 0; ok && next_item(sm, n, lane, w); ++n) {
     const int last_any = max(w.last[0], w.last[1]);
     if (lane == 0) {
-#pragma unroll
-      for (int t = 0; t < kQTiles; ++t)
-        if (ok && w.last[t] >= 0) {
-          if (q_used[t] > 0) ok = await(&sm.q_empty[t], (uint32_t)(q_used[t] - 1) & 1u, &sm.wait);
-          if (ok)
-            tma_load_tile<kTile>(sm.q[t], &p.q_map, head * p.group, w.row0 + w.tok0 + t * tile_tokens, &sm.q_full[t]);
-          ++q_used[t];
+      const auto load_q = [&](int t) {
+        if (!ok || w.last[t] < 0) return;
+        uint64_t* const full = &sm.q_full[t];
+        const uint32_t used = q_used[t]++;
+        if (used > 0) ok = await(&sm.q_empty[t], (used - 1) & 1u, &sm.wait);
+        if (ok)
+          tma_load_tile<kTile>(sm.q[t], &p.q_map, w.head * p.group, w.row0 + w.tok0 + t * tile_tokens, full);
+      };
+      for (int j = 0; ok && j <= last_any; ++j, ++tile) {
+        const uint32_t stage = tile % kStages, use = tile / kStages;
+        const int row = w.row0 + j * kKeys;
+        if (use > 0) ok = await(&sm.k_empty[stage], (use - 1) & 1u, &sm.wait);
+        if (ok && j != p.skip_tile) tma_load_tile<kKeys>(sm.k[stage], &p.k_map, w.head, row, &sm.k_full[stage]);
+        if (j == 0) {
+          load_q(0);
+          load_q(1);
         }
-      for (int j = 0; ok && j <= last_any; ++j, ++tiles) {
-        const int stage = tiles % kStages, use = tiles / kStages, row = w.row0 + j * kKeys;
-        if (use > 0) ok = await(&sm.k_empty[stage], (uint32_t)(use - 1) & 1u, &sm.wait);
-        if (ok && j != p.skip_tile) tma_load_tile<kKeys>(sm.k[stage], &p.k_map, head, row, &sm.k_full[stage]);
-        if (ok && use > 0) ok = await(&sm.v_empty[stage], (uint32_t)(use - 1) & 1u, &sm.wait);
-        if (ok) tma_load_tile<kKeys>(sm.v[stage], &p.v_map, head, row, &sm.v_full[stage]);
+        if (ok && use > 0) ok = await(&sm.v_empty[stage], (use - 1) & 1u, &sm.wait);
+        if (ok) tma_load_tile<kKeys>(sm.v[stage], &p.v_map, w.head, row, &sm.v_full[stage]);
       }
     }
     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-    if (!ok) break;
   }
   if (lane != 0 || !*(volatile int*)&sm.wait.abort) return;
   // A wait ran out somewhere.  Shared memory is given back at the end of the
   // kernel, so this thread stays until its own copies have landed (bounded: a
   // tile that was left out never lands).
   for (int b = 0; b < 2 * kStages + kQTiles; ++b) {
-    uint64_t* bar = b < kStages ? &sm.k_full[b] : b < 2 * kStages ? &sm.v_full[b - kStages] : &sm.q_full[b - 2 * kStages];
+    uint64_t* bar = b < kStages       ? &sm.k_full[b]
+                    : b < 2 * kStages ? &sm.v_full[b - kStages]
+                                      : &sm.q_full[b - 2 * kStages];
     for (int parity = 0; parity < 2; ++parity)
       for (int tries = 0; tries < 100 && !mbar_try(bar, (uint32_t)parity, 1000u); ++tries) {
       }
@@ -367,20 +406,10 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
   __syncwarp();
 }
 
-// Takes the next item; false: none is left (or a wait ran out).
-__device__ __forceinline__ bool next_item(PromptSmem& sm, int n, int lane, Item& w) {
-  const int slot = n & 1;
-  if (!await(&sm.item_full[slot], (uint32_t)(n >> 1) & 1u, &sm.wait)) return false;
-  w = sm.item[slot];
-  __syncwarp();
-  if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
-  return w.head >= 0;
-}
-
 // The warp that issues the score products, key tile by key tile for both query
 // tiles: S_t(j) as soon as the softmax has taken S_t(j - 1).
 __device__ __forceinline__ void issue_scores(PromptSmem& sm, uint32_t tmem, int lane) {
-  uint32_t items[kQTiles] = {0, 0}, issued[kQTiles] = {0, 0};
+  uint32_t q_used[kQTiles] = {0, 0}, issued[kQTiles] = {0, 0};
   uint32_t tile = 0;  // key tiles so far
   Item w;
   for (int n = 0; next_item(sm, n, lane, w); ++n) {
@@ -392,7 +421,7 @@ __device__ __forceinline__ void issue_scores(PromptSmem& sm, uint32_t tmem, int 
 #pragma unroll
       for (int t = 0; t < kQTiles; ++t) {
         if (j > w.last[t]) continue;
-        if (j == 0) await(&sm.q_full[t], items[t]++ & 1u, &sm.wait);
+        if (j == 0) await(&sm.q_full[t], q_used[t]++ & 1u, &sm.wait);
         if (issued[t] > 0) await(&sm.s_free[t], (issued[t] - 1) & 1u, &sm.wait);
         ++issued[t];
         __syncwarp();
@@ -473,32 +502,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float low, float high) {
   return r;
 }
 
-// 2^x of two values of at most about 8 on the FP32 pipe: x = n + f with n the
-// nearest integer (added and taken off again at 1.5 * 2^23, whose low bits then
-// hold n), 2^f by a polynomial that is exact at 0, n added to the exponent.
-// Below -127 the result is 0.  The coefficients are a least-maximum fit of the
-// relative error over [-1/2, 1/2]: 1.0e-4, a 39th of the half step of BF16.
-constexpr float kExp1 = 0.69328290f, kExp2 = 0.24221097f, kExp3 = 0.05500906f;
-__device__ __forceinline__ uint64_t exp2_polynomial(uint64_t x) {
-  float a, b;
-  unpack2(x, a, b);
-  x = pack2(fmaxf(a, -127.f), fmaxf(b, -127.f));
-  const uint64_t big = pack2(12582912.f, 12582912.f), minus_big = pack2(-12582912.f, -12582912.f);
-  const uint64_t shifted = add2(x, big);
-  const uint64_t whole = add2(shifted, minus_big);
-  const uint64_t f = fma2(whole, pack2(-1.f, -1.f), x);
-  uint64_t y = fma2(f, pack2(kExp3, kExp3), pack2(kExp2, kExp2));
-  y = fma2(f, y, pack2(kExp1, kExp1));
-  y = fma2(f, y, pack2(1.f, 1.f));
-  float na, nb;
-  unpack2(shifted, na, nb);
-  unpack2(y, a, b);
-  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23)),
-               __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23)));
-}
-
-// Loads or stores kCount 32-bit columns of this thread's lane, in pieces of 32,
-// 16 and 8; the caller waits.
+// Loads or stores kCount 32-bit columns of this thread's lane; the caller waits.
 template <int kCount>
 __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t* r) {
   if constexpr (kCount >= 32) {
@@ -524,70 +528,70 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t* r) {
   }
 }
 
-// Softmax warps of query tile `mine`: a thread has one query row and, of the
-// tile's columns, part `part` of kParts.
-__device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int mine, int part,
-                                               int row) {
-  constexpr int kCols = kKeys / kParts, kOCols = kTile / kParts;
+// Scores of the columns behind `visible` become -inf, in place.  A rolled loop
+// over the few pieces that the diagonal crosses, in front of the one copy of the
+// softmax: a second, masked copy of that was fetched anew by every item and its
+// steps took twice as long.
+__device__ __forceinline__ void hide_later(uint32_t tmem_s, int visible) {
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 16) {
+    if (__all_sync(0xffffffffu, visible >= c + 15)) continue;
+    uint32_t s[16];
+    tmem_load16_async(tmem_s + (uint32_t)c, s);
+    tmem_wait_loads();
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      if (c + x > visible) s[x] = 0xff800000u;
+    tmem_store16(tmem_s + (uint32_t)c, s);
+  }
+  tmem_wait_stores();
+}
+
+// Softmax warps of query tile `mine`: thread = query row.
+__device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int mine, int row) {
   const int lane = row & 31, rows = row >> 5;
   const uint32_t lanes = (uint32_t)(32 * rows) << 16;
-  const uint32_t tmem_s = tmem + lanes + kTmemS + (uint32_t)(mine * kKeys + part * kCols);
-  const uint32_t tmem_p = tmem + lanes + kTmemP + (uint32_t)(mine * (kKeys / 2) + part * (kCols / 2));
-  const uint32_t tmem_o = tmem + lanes + (uint32_t)(mine * kTile + part * kOCols);
+  const uint32_t tmem_s = tmem + lanes + kTmemS + (uint32_t)(mine * kKeys);
+  const uint32_t tmem_p = tmem + lanes + kTmemP + (uint32_t)(mine * (kKeys / 2));
+  const uint32_t tmem_o = tmem + lanes + (uint32_t)(mine * kTile);
   const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
-  uint32_t s_used = 0, sums = 0, met = 0;
-  // What the other thread of the row has.
-  const auto exchange = [&](float x) {
-    float* at = sm.half_row[met & 1][mine][0] + row;
-    ++met;
-    at[part * kTile] = x;
-    asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * mine + rows) : "memory");
-    return at[(part ^ 1) * kTile];
-  };
-  // Whether any thread of these rows asks for it.
-  const auto any_row = [&](bool asks) -> bool {
-    if constexpr (kParts == 1) return __any_sync(0xffffffffu, asks);
-    uint32_t any;
-    asm volatile(
-        "{\n\t.reg .pred q, r;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.or.pred r, %2, 64, q;\n\tselp.b32 %0, 1, 0, r;\n\t}"
-        : "=r"(any)
-        : "r"((uint32_t)asks), "r"(1 + 4 * mine + rows)
-        : "memory");
-    return any != 0;
+  uint32_t s_used = 0, sums = 0;
+  // Tile 0's warp and tile 1's of the same rows sit on one scheduler and take
+  // turns at the exponentials, tile 0 first: side by side both would be slow,
+  // and the tensor cores would wait for both.
+  uint32_t turns = 0;
+  const auto take_turn = [&] {
+    if (mine == 1 || turns > 0) await(&sm.turn[mine][rows], (mine == 1 ? turns : turns - 1) & 1u, &sm.wait);
+    ++turns;
   };
   Item w;
   for (int n = 0; next_item(sm, n, lane, w); ++n) {
     const int my_last = w.last[mine];
     // Rows past the prompt compute like its last token.
-    const int position = min(w.tok0 + (mine * kTile + row) / p.group, w.length - 1) - part * kCols;
+    const int position = min(w.tok0 + ((mine * kTile + row) >> p.group_log2), w.length - 1);
     // Key tiles below this one are seen whole by every row.
-    const int first_masked = (w.tok0 + mine * kTile / p.group + 1) / kKeys;
+    const int first_masked = (w.tok0 + (mine * kTile >> p.group_log2) + 1) / kKeys;
     float ref = 0.f;  // reference point of the exponentials
     uint64_t row_sum[2] = {0, 0};
-    const auto step = [&](int j, auto masked) {
+#pragma unroll 1
+    for (int j = 0; j <= my_last; ++j) {
       await(&sm.s_ready[mine], s_used & 1u, &sm.wait);
       ++s_used;
       tmem_acquire();
-      uint32_t s[kCols];
-      tmem_load<kCols>(tmem_s, s);
+      if (j >= first_masked) hide_later(tmem_s, position - j * kKeys);
+      uint32_t s[kKeys];
+      tmem_load<kKeys>(tmem_s, s);
       tmem_wait_loads();
       tmem_release();
-      mbar_arrive(&sm.s_free[mine]);
-      if constexpr (decltype(masked)::value) {
-        const int visible = position - j * kKeys;  // columns 0..visible of this part count
-#pragma unroll
-        for (int x = 0; x < kCols; ++x)
-          if (x > visible) s[x] = 0xff800000u;
-      }
+      arrive_warp(&sm.s_free[mine], lane);
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int x = 0; x < kCols; x += 2)
+      for (int x = 0; x < kKeys; x += 2)
         top[(x >> 1) & 3] = max3(top[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
       // The scale is positive, so the largest raw score gives the largest scaled one.
       float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
       // The reference follows the running maximum once that is kRescaleSlack above it.
-      if (any_row(j == 0 || !(tile_max <= ref + kRescaleSlack))) {
-        if constexpr (kParts == 2) tile_max = max3(tile_max, exchange(tile_max), tile_max);
+      if (__any_sync(0xffffffffu, j == 0 || !(tile_max <= ref + kRescaleSlack))) {
         // An infinite or NaN maximum makes the whole row NaN (its output is then
         // computed again, key by key).
         if (!(tile_max < INFINITY)) tile_max = NAN;
@@ -604,7 +608,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
           await(&sm.p_free[mine], s_used & 1u, &sm.wait);  // the O product before this one is done
           tmem_acquire();
 #pragma unroll 1
-          for (int c = 0; c < kOCols; c += 16) {
+          for (int c = 0; c < kTile; c += 16) {
             uint32_t o[16];
             tmem_load16_async(tmem_o + (uint32_t)c, o);
             tmem_wait_loads();
@@ -615,48 +619,36 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
         }
       }
       const uint64_t minus_ref = pack2(-ref, -ref);
-      uint32_t packed[kCols / 2];
+      take_turn();
+      uint32_t packed[kKeys / 2];
 #pragma unroll
-      for (int i = 0; i < kCols / 2; ++i) {  // pairs of columns
-        uint64_t x = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, minus_ref);
+      for (int i = 0; i < kKeys / 2; ++i) {  // pairs of columns
         float a, b;
-        // A quarter of the pairs on the FP32 pipe: the special-function unit alone
-        // would take as long as both products.
-        if (i % 4 == 1) {
-          x = exp2_polynomial(x);
-          unpack2(x, a, b);
-        } else {
-          unpack2(x, a, b);
-          a = ex2(a);
-          b = ex2(b);
-          x = pack2(a, b);
-        }
-        row_sum[i & 1] = add2(row_sum[i & 1], x);
+        unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, minus_ref), a, b);
+        a = ex2(a);
+        b = ex2(b);
+        row_sum[i & 1] = add2(row_sum[i & 1], pack2(a, b));
         packed[i] = bf16_pair(a, b);
       }
+      arrive_warp(&sm.turn[mine ^ 1][rows], lane);
       if (s_used > 1) await(&sm.p_free[mine], s_used & 1u, &sm.wait);
       tmem_acquire();
-      tmem_store<kCols / 2>(tmem_p, packed);
+      tmem_store<kKeys / 2>(tmem_p, packed);
       tmem_wait_stores();
       tmem_release();
-      mbar_arrive(&sm.p_ready[mine]);
-    };
-    int j = 0;
-#pragma unroll 1
-    for (; j < min(first_masked, my_last + 1); ++j) step(j, std::false_type{});
-#pragma unroll 1
-    for (; j <= my_last; ++j) step(j, std::true_type{});
+      arrive_warp(&sm.p_ready[mine], lane);
+    }
+    for (int j = my_last + 1; j <= w.last[mine ^ 1]; ++j) {  // the other tile goes on alone
+      take_turn();
+      arrive_warp(&sm.turn[mine ^ 1][rows], lane);
+    }
     if (my_last < 0) continue;
     float a, b;
     unpack2(add2(row_sum[0], row_sum[1]), a, b);
-    a += b;
-    if constexpr (kParts == 2) a += exchange(a);
-    if (part == 0) {
-      if (sums > 0) await(&sm.sum_empty[mine], (sums - 1) & 1u, &sm.wait);
-      ++sums;
-      sm.sum[mine][row] = a;
-      mbar_arrive(&sm.sum_full[mine]);
-    }
+    if (sums > 0) await(&sm.sum_empty[mine], (sums - 1) & 1u, &sm.wait);
+    ++sums;
+    sm.sum[mine][row] = a + b;
+    arrive_warp(&sm.sum_full[mine], lane);
   }
 }
 
@@ -712,38 +704,51 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
       if (w.last[t] < 0) continue;
       await(&sm.sum_full[t], used[t] & 1u, &sm.wait);
       const float sum = sm.sum[t][row];
-      mbar_arrive(&sm.sum_empty[t]);
+      arrive_warp(&sm.sum_empty[t], lane);
       await(&sm.o_done[t], used[t] & 1u, &sm.wait);
       ++used[t];
       tmem_acquire();
       const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays NaN
-      const int of_pair = t * kTile + row, tok = w.tok0 + of_pair / p.group, g = of_pair % p.group;
-      __nv_bfloat16* dst = p.out + (int64_t)(w.row0 + tok) * p.o_token + (int64_t)(w.head * p.group + g) * p.o_head;
-      bool finite = true;
+      // Rows go out through shared memory, so that they leave in whole lines; a
+      // warp keeps to its 32 rows.
+      const uint64_t inv2 = pack2(inv, inv);
+      uint64_t stray = 0;  // becomes NaN with any infinite or NaN result
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 32) {
         uint32_t o[32];
         tmem_load32(tmem_o + (uint32_t)(t * kTile + c), o);
-        if (tok < w.length) {
 #pragma unroll
-          for (int ch = 0; ch < 4; ++ch) {
-            uint32_t packed[4];
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t packed[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float a = __uint_as_float(o[8 * ch + 2 * x]) * inv, b = __uint_as_float(o[8 * ch + 2 * x + 1]) * inv;
-              finite &= fabsf(a) < INFINITY && fabsf(b) < INFINITY;
-              packed[x] = bf16_pair(a, b);
-            }
-            *reinterpret_cast<uint4*>(dst + c + 8 * ch) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          for (int x = 0; x < 4; ++x) {
+            const uint64_t y = fma2(pack2(__uint_as_float(o[8 * ch + 2 * x]), __uint_as_float(o[8 * ch + 2 * x + 1])), inv2, 0);
+            stray = fma2(y, 0, stray);
+            float a, b;
+            unpack2(y, a, b);
+            packed[x] = bf16_pair(a, b);
           }
+          *reinterpret_cast<uint4*>(sm.o + tile_chunk(row, c + 8 * ch)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
         }
       }
       tmem_release();
+      arrive_warp(&sm.o_free[t], lane);
+      const int first_row = t * kTile + (row & ~31);
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 2) {
+        const int r = first_row + i + (lane >> 4), tok = w.tok0 + (r >> p.group_log2);
+        if (tok >= w.length) break;
+        *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + tok) * p.o_token +
+                                  (int64_t)(w.head * p.group + (r & (p.group - 1))) * p.o_head + 8 * (lane & 15)) =
+            *reinterpret_cast<const uint4*>(sm.o + tile_chunk(r & (kTile - 1), 8 * (lane & 15)));
+      }
+      float a, b;
+      unpack2(stray, a, b);
+      const bool finite = (a == 0.f && b == 0.f) || w.tok0 + ((t * kTile + row) >> p.group_log2) >= w.length;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.o_free[t]);
       for (uint32_t again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
-        const int r = t * kTile + row - lane + __ffs(again) - 1;
-        prompt_row(p, w.row0, w.tok0 + r / p.group, w.head, w.head * p.group + r % p.group, lane);
+        const int r = first_row + __ffs(again) - 1;
+        prompt_row(p, w.row0, w.tok0 + (r >> p.group_log2), w.head, w.head * p.group + (r & (p.group - 1)), lane);
       }
     }
   }
@@ -773,13 +778,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
       mbar_init(&sm.q_full[t], 1);
       mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_ready[t], 1);
-      mbar_init(&sm.s_free[t], kParts * kTile);
-      mbar_init(&sm.p_ready[t], kParts * kTile);
+      mbar_init(&sm.s_free[t], 4);  // warps, as all counts below
+      mbar_init(&sm.p_ready[t], 4);
       mbar_init(&sm.p_free[t], 1);
-      mbar_init(&sm.sum_full[t], kTile);
-      mbar_init(&sm.sum_empty[t], kTile);
+      for (int i = 0; i < 4; ++i) mbar_init(&sm.turn[t][i], 1);
+      mbar_init(&sm.sum_full[t], 4);
+      mbar_init(&sm.sum_empty[t], kResultWarps);
       mbar_init(&sm.o_done[t], 1);
-      mbar_init(&sm.o_free[t], 4);  // result warps
+      mbar_init(&sm.o_free[t], kResultWarps);
     }
     mbar_init(&sm.drained[0], 1);
     mbar_init(&sm.drained[1], 1);
@@ -803,7 +809,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
 
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    prompt_softmax(p, sm, tmem, warp / (4 * kParts), (warp >> 2) % kParts, tid & (kTile - 1));
+    prompt_softmax(p, sm, tmem, warp >> 2, tid & (kTile - 1));
   } else if (warp < kScoreWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kResultRegs));
     prompt_results(p, sm, tmem, tid & (kTile - 1));
@@ -812,6 +818,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     if (warp == kScoreWarp) issue_scores(sm, tmem, lane);
     if (warp == kValueWarp) issue_values(sm, tmem, lane);
     if (warp == kLoadWarp) prompt_load(p, sm, lane);
+    if (warp == kItemWarp) prompt_items(p, sm, lane);
   }
   tmem_release();
   __syncthreads();
@@ -910,6 +917,7 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.tokens = (int)tokens;
   p.kv_heads = kv_heads;
   p.group = group;
+  p.group_log2 = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_limit = wait_debug().limit;
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
