@@ -66,6 +66,9 @@ CASES = [
     (40, 6, 3, 120, True, None, torch.int32, (1 << 31) - 1),
     (1000, 32, 32, 128, False, torch.bfloat16, torch.int64, 32768),
     (5, 4, 2, 0, False, torch.bfloat16, torch.int64, 100),
+    # From 65,536 rows on a half warp takes sixteen heads of a token.
+    (2107, 30, 3, 64, True, torch.float32, torch.int64, 32768),
+    (901, 73, 1, 128, False, None, torch.int32, 4096),
 ]
 
 
@@ -227,6 +230,11 @@ LAYOUTS = {
     "continued block": [[([7, 8], 0, 21)], [([7, 8], 21, 200)]],
     "decode batch": [[([b], 0, 10 + 3 * b) for b in range(16)], [([b], 10 + 3 * b, 1) for b in range(16)]],
     "many rows": [[([b], 0, 1 + 11 * b % T) for b in range(20)]],
+    # More than 384 tokens: groups of sixteen that start anywhere among the input's sixteens, beside single tokens.
+    "long rows": [
+        [([1], 0, 5), ([2, 3, 4, 5], 0, 3 * T + 37), ([6], 0, 16), ([7], 0, 1), ([8, 9], 0, T + 2)],
+        [([1], 5, 100), ([5, 13], 3 * T + 37 - 3 * T, 98), ([10, 11, 12], 0, 301), ([9], 2, 1)],
+    ],
 }
 
 
@@ -241,7 +249,7 @@ def test_append_equals_norm_rotary_then_write(name, h, group) -> None:
     for step, rows in enumerate(LAYOUTS[name]):
         pos = [p for _, start, n in rows for p in range(start, start + n)]
         slots = [blocks[p // T] * T + p % T for blocks, start, n in rows for p in range(start, start + n)]
-        if name in ("shifted rows", "decode batch"):  # unstored tokens before, inside and behind
+        if name in ("shifted rows", "decode batch", "long rows"):  # unstored tokens before, inside and behind
             pos, slots = [9] + pos[:3] + [0] + pos[3:] + [1, 2], [-1] + slots[:3] + [-7] + slots[3:] + [-1, -1]
         if name == "whole blocks":  # input order broken inside a group of sixteen
             pos[32:34], slots[32:34] = pos[33:31:-1], slots[33:31:-1]
