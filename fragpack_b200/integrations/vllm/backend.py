@@ -26,6 +26,11 @@ decompresses into the workspace and calls vLLM's FlashAttention-3, which is
 SM90-only; that two-step path is kept as ``run_layer(..., fused_prefill=False)``
 with torch SDPA per request in FlashAttention's place); the decode workspace
 is sized by this package's ``workspace_elems``.
+
+Two things the reference leaves to its engine can be done here: a layer's heads
+are normed and rotated on the way into the store (``run_layer(...,
+transform=)``), and prefill rows that are whole prompts attend straight to the
+keys and values of the step (``FRAGPACK_PROMPT_ATTENTION=1``, off by default).
 """
 
 from __future__ import annotations
@@ -47,6 +52,8 @@ from fragpack_b200.ops.fused_attn_decode import (
 )
 from fragpack_b200.ops.hbm_kv import BLOCK_TOKENS, HEAD_DIM, HbmKvStore, page_bytes, register_store
 from fragpack_b200.ops.prefill_attn import prefill_attention as fused_prefill_attention
+from fragpack_b200.ops.prompt_attn import prompt_attention
+from fragpack_b200.ops.rotary import Rotary, norm_rotary
 
 _POLL_EVERY = 16
 _LOG_EVERY = 4096
@@ -71,6 +78,7 @@ class PrefillGroup:
         tok1: One past the last token.
         max_seqlen_q: Longest query of the group.
         max_seqlen_k: Longest context of the group.
+        whole: Every row's queries are its whole context (nothing was cached).
     """
 
     src_blocks: torch.Tensor
@@ -82,11 +90,34 @@ class PrefillGroup:
     tok1: int
     max_seqlen_q: int
     max_seqlen_k: int
+    whole: bool = False
+
+
+@dataclass(frozen=True)
+class HeadTransform:
+    """What a layer does to its projected query and key heads before the cache.
+
+    Attributes:
+        rotary: The position rotation.
+        positions: int64 or int32 ``[T]`` positions of the step's tokens.
+        query_weight, key_weight: ``[128]`` weights of the RMS norms, or None.
+        eps: Added to the mean square of the norms.
+    """
+
+    rotary: Rotary
+    positions: torch.Tensor
+    query_weight: torch.Tensor | None = None
+    key_weight: torch.Tensor | None = None
+    eps: float = 1e-6
 
 
 @dataclass
 class FragPackMetadata:
-    """Per-step metadata shared by every layer (``backend.py:120-156``)."""
+    """Per-step metadata shared by every layer (``backend.py:120-156``).
+
+    ``prompt_attention``: attend prefill groups that are whole prompts over the
+    step's own keys and values (:func:`~fragpack_b200.ops.prompt_attn.prompt_attention`).
+    """
 
     store: HbmKvStore
     layer_tables: list[RecordTables]
@@ -103,6 +134,7 @@ class FragPackMetadata:
     prefills: list[PrefillGroup]
     wk: torch.Tensor
     wv: torch.Tensor
+    prompt_attention: bool = False
 
 
 def count_closes(seq_lens: np.ndarray, query_lens: np.ndarray) -> int:
@@ -123,6 +155,7 @@ def plan_prefill_groups(
     seq_lens: np.ndarray,
     workspace_pages: int,
     device: torch.device,
+    split_whole: bool = False,
 ) -> list[PrefillGroup]:
     """Split the prefill rows into workspace passes (``backend.py:385-446``).
 
@@ -138,11 +171,16 @@ def plan_prefill_groups(
         seq_lens: int64 ``[num_reqs]`` context lengths after this step.
         workspace_pages: Pages of the BF16 workspace.
         device: Device of the index tensors.
+        split_whole: Also close a group between rows that are whole prompts and
+            rows with cached context, so that no group mixes them.
     """
     pages = -(-np.asarray(seq_lens, np.int64) // BLOCK_TOKENS)
+    query_lens = np.asarray(query_start[1 : num_reqs + 1]) - np.asarray(query_start[:num_reqs])
+    whole = query_lens == np.asarray(seq_lens[:num_reqs])
     bounds, start, used = [], first, 0
     for row in range(first, num_reqs):
-        if used + pages[row] > workspace_pages and row > start:
+        full = used + pages[row] > workspace_pages
+        if (full or (split_whole and whole[row] != whole[start])) and row > start:
             bounds.append((start, row))
             start, used = row, 0
         used += int(pages[row])
@@ -181,6 +219,7 @@ def plan_prefill_groups(
                 tok1=int(query_start[r1]),
                 max_seqlen_q=int((query_start[r0 + 1 : r1 + 1] - query_start[r0:r1]).max()),
                 max_seqlen_k=int(np.asarray(seq_lens[r0:r1]).max()),
+                whole=bool(whole[r0:r1].all()),
             )
         )
     return groups
@@ -239,6 +278,8 @@ def run_layer(
     scale: float,
     prefill_attention: Callable[..., None] = workspace_prefill_attention,
     fused_prefill: bool = True,
+    transform: HeadTransform | None = None,
+    fused_append: bool = True,
 ) -> torch.Tensor:
     """One layer of a step: write new KV, attend, encode closed blocks (``backend.py:536-579``).
 
@@ -254,6 +295,12 @@ def run_layer(
         fused_prefill: Attend prefill rows directly over the compressed records
             (one tensor-core kernel per group, no workspace) instead of
             decompressing into the workspace first.
+        transform: Norm and rotate ``query`` and ``key`` first: ``query`` is
+            overwritten with the result, ``key`` where something after the
+            store reads it (or ``fused_append`` is false).  None: they are
+            ready for the cache.
+        fused_append: Norm, rotate and store in one kernel
+            (:meth:`HbmKvStore.append`) instead of one after the other.
 
     Returns:
         ``output``.
@@ -263,14 +310,29 @@ def run_layer(
     """
     store = md.store
     n = md.num_tokens
-    store.write(layer, key[:n], value[:n], md.slot_mapping[:n])
+    direct = [md.prompt_attention and group.whole for group in md.prefills]
+    if transform is None:
+        store.write(layer, key[:n], value[:n], md.slot_mapping[:n])
+    elif fused_append:
+        store.append(
+            layer, query[:n], key[:n], value[:n], transform.positions[:n], md.slot_mapping[:n], transform.rotary,
+            query[:n], key[:n] if any(direct) else None, transform.query_weight, transform.key_weight, transform.eps,
+        )
+    else:
+        norm_rotary(query[:n], key[:n], transform.positions[:n], transform.rotary, query[:n], key[:n],
+                    transform.query_weight, transform.key_weight, transform.eps)
+        store.write(layer, key[:n], value[:n], md.slot_mapping[:n])
     nd = md.num_decodes
     if nd:
         decode_attention(
             query[:nd], md.layer_tables[layer], md.decode_block_table, md.decode_seq_lens, scale,
             md.units, output[:nd], md.decode_workspace, replan=layer == 0,
         )
-    for group in md.prefills:
+    for group, over_prompt in zip(md.prefills, direct):
+        rows = slice(group.tok0, group.tok1)
+        if over_prompt:
+            prompt_attention(query[rows], key[rows], value[rows], group.cu_seqlens_q, scale, output[rows])
+            continue
         if fused_prefill:
             fused_prefill_attention(
                 query[group.tok0 : group.tok1], md.layer_tables[layer], group.store_block_table,
@@ -408,6 +470,7 @@ def _bind_vllm() -> dict[str, Any]:
             self.tables = load_tables(path, device, heads)
             if self.tables.plut.shape[2] != self.kv_heads:
                 raise ValueError(f"FragPack tables {path} do not cover KV heads {heads.start}..{heads.stop}")
+            self.prompt_attention = os.environ.get("FRAGPACK_PROMPT_ATTENTION", "0") == "1"
             self.store: HbmKvStore | None = None
             self.store_key: tuple[int, int] | None = None
             self.layer_tables: list[RecordTables] = []
@@ -440,7 +503,8 @@ def _bind_vllm() -> dict[str, Any]:
             prefills: list[PrefillGroup] = []
             if npf and not capture:
                 prefills = plan_prefill_groups(cam.block_table_tensor, nd, num_reqs, qsl, seq,
-                                               self.workspace_pages, self.device)
+                                               self.workspace_pages, self.device,
+                                               split_whole=self.prompt_attention)
             return FragPackMetadata(
                 store=store, layer_tables=self.layer_tables, layer_index=self.layer_index,
                 last_layer=len(self.layer_names) - 1, slot_mapping=cam.slot_mapping,
@@ -448,7 +512,7 @@ def _bind_vllm() -> dict[str, Any]:
                 decode_seq_lens=cam.seq_lens[:nd],
                 units=decode_units(max(nd, 1), self.kv_heads, self.num_sms),
                 decode_workspace=self.decode_workspace, max_close=max_close, prefills=prefills,
-                wk=self.wk, wv=self.wv,
+                wk=self.wk, wv=self.wv, prompt_attention=self.prompt_attention,
             )
 
         def _store(self) -> HbmKvStore:
@@ -571,6 +635,7 @@ __all__ = [
     "FragPackAttentionImpl",
     "FragPackMetadata",
     "FragPackMetadataBuilder",
+    "HeadTransform",
     "PrefillGroup",
     "check_impl_arguments",
     "count_closes",
