@@ -23,7 +23,7 @@
 // product in turn, and the same kernel took 3,800 cycles per 128 keys of an item
 // against 2,048 of the products.
 //
-// One persistent CTA per SM; its warps meet only through mbarriers, and every
+// One CTA per SM at a time, which goes from item to item; its warps meet only through mbarriers, and every
 // wait is bounded and reports through the status word:
 //   softmax warps  those of query tile 0, then those of tile 1 (a warp reaches
 //                  the tensor-memory lanes 32 (warp % 4) ..)
@@ -81,7 +81,9 @@ struct PromptSmem {
   __align__(1024) uint8_t v[kStages][kKeyTileBytes];
   float sum[kQTiles][kTile];  // of the probabilities of each row
   Item item[2];
-  __align__(8) uint64_t item_full[2], item_empty[2];
+  __align__(16) uint8_t block[16];  // answer to the request for a block
+  __align__(8) uint64_t block_full;
+  uint64_t item_full[2], item_empty[2];
   uint64_t q_full[kQTiles], q_empty[kQTiles];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_ready[kQTiles], s_free[kQTiles];         // S product done; S read
@@ -252,17 +254,20 @@ __device__ __forceinline__ Prompt load_prompt(const PromptParams& p, int r) {
   return x;
 }
 
-// Picks the CTA's items, one warp.  Items come in the order "all prompts' pairs
-// i, from the largest i down" (for every KV head), so that the longest are under
-// way first, and CTAs take them forwards and backwards in turn, so that the sums
-// of what they get stay close.  The warp walks down the levels i; `above` counts
-// the pairs of the levels done.
-__device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& sm, int lane) {
+// Finds items by their number, one warp.  They are numbered in the order "all
+// prompts' pairs i, from the largest i down" (for every KV head), so that the
+// longest are under way first; the warp walks down the levels i (numbers must
+// not fall from call to call), and `above` counts the pairs of the levels done.
+struct ItemPicker {
+  const PromptParams& p;
+  const int lane;
   Prompt kept[kKept];
-#pragma unroll
-  for (int g = 0; g < kKept; ++g) kept[g] = load_prompt(p, 32 * g + lane);
+  int level = -1;
+  uint32_t above = 0, here = 0;  // `here`: prompts that have a pair of this level
+
   // f(group of 32 prompts) in order, until it returns true (f is warp-uniform).
-  const auto each_group = [&](auto&& f) {
+  template <typename F>
+  __device__ __forceinline__ void each_group(F&& f) {
 #pragma unroll
     for (int g = 0; g < kKept; ++g) {
       if (32 * g >= p.prompts) return;
@@ -271,62 +276,130 @@ __device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& 
 #pragma unroll 1
     for (int r = 32 * kKept; r < p.prompts; r += 32)
       if (f(load_prompt(p, r + lane))) return;
-  };
-  int level = 0, above = 0, here = 0;  // `here`: prompts that have a pair of this level
-  const auto count_level = [&] {
+  }
+  __device__ __forceinline__ void count_level() {
     here = 0;
     each_group([&](const Prompt& x) {
-      here += __popc(__ballot_sync(0xffffffffu, x.pairs > level));
+      here += (uint32_t)__popc(__ballot_sync(0xffffffffu, x.pairs > level));
       return false;
     });
-  };
-  each_group([&](const Prompt& x) {
-    level = max(level, (int)__reduce_max_sync(0xffffffffu, (unsigned)x.pairs));
-    return false;
-  });
-  --level;
-  if (level >= 0) count_level();
-  const int tile_tokens = kTile >> p.group_log2;
-  for (int n = 0;; ++n) {
-    const int slot = n & 1;
-    const int64_t at = (int64_t)n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    const int64_t x = at / p.kv_heads;  // pair of every head
+  }
+  __device__ __forceinline__ ItemPicker(const PromptParams& params, int lane_) : p(params), lane(lane_) {
+#pragma unroll
+    for (int g = 0; g < kKept; ++g) kept[g] = load_prompt(p, 32 * g + lane);
+    uint32_t most = 0;
+    each_group([&](const Prompt& x) {
+      most = max(most, __reduce_max_sync(0xffffffffu, (unsigned)x.pairs));
+      return false;
+    });
+    level = (int)most - 1;
+    if (level >= 0) count_level();
+  }
+  // Item number `at`; head -1: there are fewer.
+  __device__ __forceinline__ Item item(uint32_t at) {
+    const uint32_t x = at / (uint32_t)p.kv_heads;  // pair of every head
     while (level >= 0 && x >= above + here) {
       above += here;
       if (--level >= 0) count_level();
     }
+    const int tile_tokens = kTile >> p.group_log2;
     Item w;
     w.head = -1;
+    w.row0 = w.length = 0;
     w.tok0 = max(level, 0) * kQTiles * tile_tokens;
     w.last[0] = w.last[1] = -1;
-    if (level >= 0) {
-      w.head = (int)(at % p.kv_heads);
-      int rank = (int)(x - above);
-      each_group([&](const Prompt& of) {
-        const uint32_t have = __ballot_sync(0xffffffffu, of.pairs > level);
-        const int count = __popc(have);
-        if (rank >= count) {
-          rank -= count;
-          return false;
-        }
-        const int src = __fns(have, 0, rank + 1);
-        w.row0 = __shfl_sync(0xffffffffu, of.row0, src);
-        w.length = __shfl_sync(0xffffffffu, of.length, src);
-        return true;
-      });
-#pragma unroll
-      for (int t = 0; t < kQTiles; ++t) {
-        const int t0 = w.tok0 + t * tile_tokens;
-        if (t0 < w.length) w.last[t] = (min(t0 + tile_tokens, w.length) - 1) / kKeys;
+    if (level < 0) return w;
+    w.head = (int)(at % (uint32_t)p.kv_heads);
+    int rank = (int)(x - above);
+    each_group([&](const Prompt& of) {
+      uint32_t have = __ballot_sync(0xffffffffu, of.pairs > level);
+      const int count = __popc(have);
+      if (rank >= count) {
+        rank -= count;
+        return false;
       }
+      for (; rank > 0; --rank) have &= have - 1;
+      const int src = __ffs(have) - 1;
+      w.row0 = __shfl_sync(0xffffffffu, of.row0, src);
+      w.length = __shfl_sync(0xffffffffu, of.length, src);
+      return true;
+    });
+#pragma unroll
+    for (int t = 0; t < kQTiles; ++t) {
+      const int t0 = w.tok0 + t * tile_tokens;
+      if (t0 < w.length) w.last[t] = (min(t0 + tile_tokens, w.length) - 1) / kKeys;
     }
-    if (n >= 2 && !await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) return;
+    return w;
+  }
+};
+
+// Every item has a block of the grid.  A CTA does its own and then takes over
+// blocks that have not started yet (cluster launch control), in their order, so
+// that whoever is done first goes on first.  The next block is asked for once
+// the item before the last one taken is on its way out: asked for earlier, it
+// would be bound to a CTA that may be late.
+__device__ __forceinline__ void ask_for_block(PromptSmem& sm, int lane) {
+  if (lane == 0) {
+    mbar_expect_tx(&sm.block_full, 16);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the answer before was read
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+            smem_addr(sm.block)),
+        "r"(smem_addr(&sm.block_full))
+        : "memory");
+  }
+  __syncwarp();
+}
+// The block's number; false: none is left.
+__device__ __forceinline__ bool block_taken(PromptSmem& sm, uint32_t& number) {
+  uint32_t taken;
+  asm volatile(
+      "{\n\t.reg .b128 answer;\n\t.reg .pred p;\n\tld.shared.b128 answer, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, answer;\n\t}"
+      : "=r"(taken), "=r"(number)
+      : "r"(smem_addr(sm.block))
+      : "memory");
+  __syncwarp();
+  return taken != 0;
+}
+
+__device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& sm, int lane) {
+  ItemPicker picker(p, lane);
+  uint32_t number = blockIdx.x, asked = 0;
+  bool more = true, answered = true;  // `number` is a block of this CTA's
+  for (int n = 0;; ++n) {
+    const int slot = n & 1;
+    if (n >= 2 && !await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) break;
+    if (n > 0) {
+      ask_for_block(sm, lane);
+      answered = await(&sm.block_full, asked++ & 1u, &sm.wait);
+      if (!answered) break;
+      more = block_taken(sm, number);
+    }
+    Item w;
+    w.head = -1;
+    if (more) w = picker.item(number);
     if (lane == 0) {
       sm.item[slot] = w;
       mbar_arrive(&sm.item_full[slot]);
     }
     __syncwarp();
-    if (w.head < 0) return;
+    if (w.head < 0) break;
+  }
+  // Blocks that are left have no item (or a wait ran out, and the call is
+  // invalid): they are taken all the same, beside the last items, so that none of
+  // them has to start.
+  while (more) {
+    if (answered) {
+      ask_for_block(sm, lane);
+      ++asked;
+    }
+    answered = false;
+    for (int tries = 0; tries < 1000 && !answered; ++tries) answered = mbar_try(&sm.block_full, (asked - 1) & 1u, 1000u);
+    answered = __all_sync(0xffffffffu, answered);
+    if (!answered) return;
+    more = block_taken(sm, number);
   }
 }
 
@@ -733,14 +806,26 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
       }
       tmem_release();
       arrive_warp(&sm.o_free[t], lane);
-      const int first_row = t * kTile + (row & ~31);
-#pragma unroll 4
-      for (int i = 0; i < 32; i += 2) {
-        const int r = first_row + i + (lane >> 4), tok = w.tok0 + (r >> p.group_log2);
-        if (tok >= w.length) break;
-        *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + tok) * p.o_token +
-                                  (int64_t)(w.head * p.group + (r & (p.group - 1))) * p.o_head + 8 * (lane & 15)) =
-            *reinterpret_cast<const uint4*>(sm.o + tile_chunk(r & (kTile - 1), 8 * (lane & 15)));
+      // Two rows at a time, 16 bytes a lane; the next two are two heads on, or in
+      // the next token (the second next with one head).
+      const int first_row = t * kTile + (row & ~31), mine = first_row + (lane >> 4);
+      int tok = w.tok0 + (mine >> p.group_log2), g = mine & (p.group - 1);
+      const uint8_t* line[4];  // rows of a swizzled group of eight
+#pragma unroll
+      for (int i = 0; i < 4; ++i) line[i] = sm.o + tile_chunk((row & ~31) + 2 * i + (lane >> 4), 8 * (lane & 15));
+      __nv_bfloat16* dst =
+          p.out + (int64_t)(w.row0 + tok) * p.o_token + (int64_t)(w.head * p.group + g) * p.o_head + 8 * (lane & 15);
+      const int64_t to_head = 2 * p.o_head, to_token = p.group == 1 ? 2 * p.o_token : p.o_token - (p.group - 2) * p.o_head;
+      const int tokens = p.group == 1 ? 2 : 1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (tok < w.length)
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(line[i & 3] + (i >> 2) * 1024);
+        g += 2;
+        const bool on = g >= p.group;
+        dst += on ? to_token : to_head;
+        tok += on ? tokens : 0;
+        g = on ? g & (p.group - 1) : g;
       }
       float a, b;
       unpack2(stray, a, b);
@@ -787,6 +872,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
       mbar_init(&sm.o_done[t], 1);
       mbar_init(&sm.o_free[t], kResultWarps);
     }
+    mbar_init(&sm.block_full, 1);
     mbar_init(&sm.drained[0], 1);
     mbar_init(&sm.drained[1], 1);
     sm.wait.abort = 0;
@@ -802,6 +888,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == kLoadWarp && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.q_map : lane == 1 ? &p.k_map : &p.v_map) : "memory");
   tmem_release();
   __syncthreads();
   tmem_acquire();
@@ -923,7 +1011,9 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
   // Every prompt has at most one pair of tiles that is not full.
   const int64_t items = (tokens / (kQTiles * tile_tokens) + prompts) * kv_heads;
-  prompt_attn_kernel<<<(unsigned)std::min<int64_t>(items, device_sms()), kPromptThreads, smem, (cudaStream_t)stream>>>(p);
+  FP_REQUIRE(items < (1LL << 31), "too much work for one call (%lld tokens, %d prompts, %d KV heads)", (long long)tokens,
+             prompts, kv_heads);
+  prompt_attn_kernel<<<(unsigned)items, kPromptThreads, smem, (cudaStream_t)stream>>>(p);
   FP_LAUNCH_CHECK("prompt_attn_kernel");
   return FP_OK;
 }
