@@ -379,26 +379,36 @@ class HbmKvStore:
         Async/thread-safety:
             One kernel on the current stream; CUDA-graph safe.
         """
-        self._require_device()
-        tokens, device = key.shape[0], self.counters.get_device()
+        device = self.counters.get_device()
+        if device < 0:
+            self._require_device()
+        tokens = key.shape[0]
         q = head_set("query", query, query_out, tokens, device)
         k = head_set("key", key, key_out, tokens, device)
         v_stride = value.stride()
-        if k.heads != self.kv_heads or value.shape != key.shape or v_stride[2] != 1:
-            raise RuntimeError(f"key and value must be [N, {self.kv_heads}, 128] with a contiguous head dim")
-        if value.dtype != torch.bfloat16 or value.get_device() != device:
-            raise RuntimeError(f"value must be bfloat16 on cuda:{device}")
-        if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != tokens:
-            raise RuntimeError(f"slot_mapping must be int64 [{tokens}]")
-        if not slot_mapping.is_contiguous() or slot_mapping.get_device() != device:
-            raise RuntimeError(f"slot_mapping must be contiguous on cuda:{device}")
-        qw, kw, f32, pos, pos64 = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
+        if (
+            k.heads != self.kv_heads
+            or value.shape != key.shape
+            or v_stride[2] != 1
+            or value.dtype is not torch.bfloat16
+            or value.get_device() != device
+        ):
+            raise RuntimeError(
+                f"key and value must be bfloat16 [N, {self.kv_heads}, 128] on cuda:{device} with a contiguous head dim"
+            )
+        if (
+            slot_mapping.dtype is not torch.int64
+            or slot_mapping.shape != (tokens,)
+            or not slot_mapping.is_contiguous()
+            or slot_mapping.get_device() != device
+        ):
+            raise RuntimeError(f"slot_mapping must be contiguous int64 [{tokens}] on cuda:{device}")
+        operands = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
         with on_device(device):
             check(
                 extension().fp_hbm_append(
-                    self._store_ref, ctypes.byref(q), ctypes.byref(k), value.data_ptr(), v_stride[0],
-                    v_stride[1], qw, kw, f32, pos, pos64, slot_mapping.data_ptr(), tokens,
-                    ctypes.byref(rotary._native), float(eps), layer, stream_ptr(),
+                    self._store_ref, ctypes.byref(q), ctypes.byref(k), value.data_ptr(), v_stride[0], v_stride[1],
+                    *operands, slot_mapping.data_ptr(), tokens, rotary._ref, eps, layer, stream_ptr(),
                 )
             )
 

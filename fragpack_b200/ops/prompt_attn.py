@@ -52,8 +52,10 @@ def prompt_attention(
     Async/thread-safety:
         One kernel on the current CUDA stream; CUDA-graph safe; allocates nothing.
     """
-    require_cuda(q, "q")
-    q_shape, kv_shape, device = q.shape, k.shape, q.get_device()
+    device = q.get_device()
+    if device < 0:
+        require_cuda(q, "q")
+    q_shape, kv_shape = q.shape, k.shape
     if len(q_shape) != 3 or len(kv_shape) != 3 or kv_shape[1] == 0:
         raise RuntimeError("q, k and v must be [T, heads, 128]")
     tokens, kv_heads = kv_shape[0], kv_shape[1]
@@ -65,20 +67,20 @@ def prompt_attention(
     if out.shape != q_shape:
         raise RuntimeError("out must have the shape of q")
     rows = []
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+    for t in (q, k, v, out):
         stride = t.stride()
-        if t.dtype != torch.bfloat16 or t.get_device() != device or stride[2] != 1:
-            raise RuntimeError(f"{name} must be bfloat16 on cuda:{device} with a contiguous head dim")
+        if t.dtype is not torch.bfloat16 or t.get_device() != device or stride[2] != 1:
+            raise RuntimeError(f"q, k, v and out must be bfloat16 on cuda:{device} with a contiguous head dim")
         rows.append((t.data_ptr(), stride[0], stride[1]))
-    if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() == 0 or not starts.is_contiguous():
+    if starts.dtype is not torch.int32 or starts.dim() != 1 or not starts.is_contiguous() or starts.numel() == 0:
         raise RuntimeError("starts must be contiguous int32 [R + 1]")
     if starts.get_device() != device:
         raise RuntimeError(f"starts must be on cuda:{device}")
     with on_device(device):
         check(
             extension().fp_prompt_attention(
-                *rows[0], *rows[1], *rows[2], starts.data_ptr(), starts.numel() - 1, tokens, *rows[3], kv_heads,
-                group, float(scale), stream_ptr(),
+                *rows[0], *rows[1], *rows[2], starts.data_ptr(), starts.shape[0] - 1, tokens, *rows[3], kv_heads,
+                group, scale, stream_ptr(),
             )
         )
 

@@ -15,7 +15,7 @@ position and no table of angles is kept.
 
 from __future__ import annotations
 
-import ctypes
+from ctypes import byref
 from dataclasses import dataclass, field
 import math
 from typing import Any
@@ -117,6 +117,7 @@ class Rotary:
     interleaved: bool
     factor: float
     _native: FpRotary = field(repr=False, compare=False)
+    _ref: Any = field(repr=False, compare=False)  # by reference, made once
 
 
 def make_rotary(
@@ -160,26 +161,38 @@ def make_rotary(
     bits = np.array(fractions + [0] * (not fractions), dtype=np.uint64).view(np.int64)
     turns = torch.from_numpy(bits).to(device)
     native = FpRotary(turns=turns.data_ptr(), rot_dim=rot_dim, interleaved=int(bool(interleaved)), factor=factor)
-    return Rotary(turns, rot_dim, bool(interleaved), factor, native)
+    return Rotary(turns, rot_dim, bool(interleaved), factor, native, byref(native))
 
 
+_BF16, _FP32, _INT64, _INT32 = torch.bfloat16, torch.float32, torch.int64, torch.int32
+
+
+# These checks are most of a small call's host time, so the sound case takes one
+# comparison each and the messages are found afterwards.
 def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: int) -> FpHeads:
     """Check one set of heads and its result on CUDA device ``device`` and describe them to the library."""
     shape, stride = heads.shape, heads.stride()
-    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
-        raise RuntimeError(f"{name} must be [T, heads, {HEAD_DIM}] with a contiguous head dim")
-    if shape[0] != tokens:
-        raise RuntimeError(f"{name} has {shape[0]} tokens, not {tokens}")
-    if heads.dtype != torch.bfloat16 or heads.get_device() != device:
-        raise RuntimeError(f"{name} must be bfloat16 on cuda:{device}")
+    if (
+        len(shape) != 3
+        or shape[0] != tokens
+        or shape[2] != HEAD_DIM
+        or stride[2] != 1
+        or heads.dtype is not _BF16
+        or heads.get_device() != device
+    ):
+        raise RuntimeError(
+            f"{name} must be bfloat16 [{tokens}, heads, {HEAD_DIM}] on cuda:{device} with a contiguous head dim, "
+            f"not {heads.dtype} {tuple(shape)} on {heads.device} with strides {stride}"
+        )
     if out is None:
         return FpHeads(heads.data_ptr(), None, stride[0], stride[1], 0, 0, shape[1])
-    out_stride = out.stride()
-    if out.shape != shape or out_stride[2] != 1:
-        raise RuntimeError(f"{name}_out must have the shape of {name} and a contiguous head dim")
-    if out.dtype != torch.bfloat16 or out.get_device() != device:
-        raise RuntimeError(f"{name}_out must be bfloat16 on cuda:{device}")
-    return FpHeads(heads.data_ptr(), out.data_ptr(), stride[0], stride[1], out_stride[0], out_stride[1], shape[1])
+    to = out.stride()
+    if out.shape != shape or to[2] != 1 or out.dtype is not _BF16 or out.get_device() != device:
+        raise RuntimeError(
+            f"{name}_out must be bfloat16 {tuple(shape)} on cuda:{device} with a contiguous head dim, "
+            f"not {out.dtype} {tuple(out.shape)} on {out.device} with strides {to}"
+        )
+    return FpHeads(heads.data_ptr(), out.data_ptr(), stride[0], stride[1], to[0], to[1], shape[1])
 
 
 def rotary_operands(
@@ -196,29 +209,41 @@ def rotary_operands(
         Pointers of the two weights, whether they are FP32, the pointer of the
         positions and whether those are int64.
     """
-    wide = positions.dtype == torch.int64
-    if not wide and positions.dtype != torch.int32 or positions.dim() != 1 or positions.numel() != tokens:
-        raise RuntimeError(f"positions must be int64 or int32 [{tokens}]")
-    if not positions.is_contiguous() or positions.get_device() != device or rotary.turns.get_device() != device:
-        raise RuntimeError(f"positions must be contiguous and on cuda:{device}, like the rotary's frequencies")
-    q = k = dtype = None
+    kind = positions.dtype
+    if (
+        (kind is not _INT64 and kind is not _INT32)
+        or positions.shape != (tokens,)
+        or not positions.is_contiguous()
+        or positions.get_device() != device
+        or rotary.turns.get_device() != device
+    ):
+        raise RuntimeError(
+            f"positions must be contiguous int64 or int32 [{tokens}] on cuda:{device}, like the rotary's frequencies"
+        )
+    q = k = None
+    dtype = _BF16
     if query_weight is not None:
-        q, dtype = _weight(query_weight, device)
+        dtype = query_weight.dtype
+        q = _weight(query_weight, dtype, device)
     if key_weight is not None:
-        k, other = _weight(key_weight, device)
-        if dtype not in (None, other):
-            raise RuntimeError("norm weights must both be bfloat16 or both float32")
-        dtype = other
-    return q, k, int(dtype == torch.float32), positions.data_ptr(), int(wide)
+        if q is None:
+            dtype = key_weight.dtype
+        k = _weight(key_weight, dtype, device)
+    return q, k, dtype is _FP32, positions.data_ptr(), kind is _INT64
 
 
-def _weight(weight: torch.Tensor, device: int) -> tuple[int, torch.dtype]:
-    dtype = weight.dtype
-    if dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError("norm weights must both be bfloat16 or both float32")
-    if weight.dim() != 1 or weight.numel() != HEAD_DIM or not weight.is_contiguous() or weight.get_device() != device:
-        raise RuntimeError(f"norm weights must be contiguous [{HEAD_DIM}] on cuda:{device}")
-    return weight.data_ptr(), dtype
+def _weight(weight: torch.Tensor, dtype: torch.dtype, device: int) -> int:
+    if (
+        (dtype is not _BF16 and dtype is not _FP32)
+        or weight.dtype is not dtype
+        or weight.shape != (HEAD_DIM,)
+        or weight.stride(0) != 1
+        or weight.get_device() != device
+    ):
+        raise RuntimeError(
+            f"norm weights must both be bfloat16 or both float32, contiguous [{HEAD_DIM}] on cuda:{device}"
+        )
+    return weight.data_ptr()
 
 
 _NO_HEADS = FpHeads(None, None, 0, 0, 0, 0, 0)
@@ -258,18 +283,19 @@ def norm_rotary(
     Async/thread-safety:
         One kernel on the current CUDA stream; CUDA-graph safe; allocates nothing.
     """
-    require_cuda(query, "query")
+    device = query.get_device()
+    if device < 0:
+        require_cuda(query, "query")
     if (key is None) != (key_out is None):
         raise RuntimeError("key and key_out come together")
-    device, tokens = query.get_device(), query.shape[0]
+    tokens = query.shape[0]
     q = head_set("query", query, query_out, tokens, device)
     k = _NO_HEADS if key is None else head_set("key", key, key_out, tokens, device)
     operands = rotary_operands(positions, tokens, rotary, query_weight, key_weight, device)
     with on_device(device):
         check(
             extension().fp_norm_rotary(
-                ctypes.byref(q), ctypes.byref(k), *operands, tokens, ctypes.byref(rotary._native), float(eps),
-                stream_ptr(),
+                byref(q), byref(k), *operands, tokens, rotary._ref, eps, stream_ptr(),
             )
         )
 

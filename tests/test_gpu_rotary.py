@@ -246,6 +246,7 @@ def test_append_equals_norm_rotary_then_write(name, h, group) -> None:
     a, b = _store(h), _store(h)
     rotary = make_rotary(a.counters.device, 128 if h != 1 else 64, 10000.0, interleaved)
     w = torch.rand(2, DIM, device="cuda").to(torch.bfloat16) if h == 4 else (None, None)
+    seen = set()  # every block stays live: a slot given back would bring its old block's scalars along
     for step, rows in enumerate(LAYOUTS[name]):
         pos = [p for _, start, n in rows for p in range(start, start + n)]
         slots = [blocks[p // T] * T + p % T for blocks, start, n in rows for p in range(start, start + n)]
@@ -256,9 +257,10 @@ def test_append_equals_norm_rotary_then_write(name, h, group) -> None:
         n = len(slots)
         positions = torch.tensor(pos, device="cuda")
         slot_t = torch.tensor(slots, device="cuda")
-        live = np.array(sorted({s // T for s in slots if s >= 0}), np.int32)
+        touched = sorted({s // T for s in slots if s >= 0})
+        seen.update(touched)
         for s in (a, b):
-            s.prepare(slot_t, n, live)
+            s.prepare(slot_t, n, np.array(sorted(seen), np.int32))
         for layer in range(L):
             _, q, k, v = _heads(n, h * group, h, seed=10 * step + layer)
             q_out, k_out = torch.zeros_like(q), torch.zeros_like(k)
@@ -269,7 +271,7 @@ def test_append_equals_norm_rotary_then_write(name, h, group) -> None:
             assert torch.equal(q_out, want_q)
             if keep:
                 assert torch.equal(k_out, want_k)
-            assert torch.equal(_records(a, layer, live), _records(b, layer, live)), layer
+            assert torch.equal(_records(a, layer, touched), _records(b, layer, touched)), layer
         for s in (a, b):
             s.commit()
 
