@@ -56,6 +56,7 @@ constexpr int kScoreWarp = kSoftmaxWarps + kResultWarps, kValueWarp = kScoreWarp
 constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kResultWarps + 4);  // whole warpgroups
 constexpr int kItemReaders = kLoadWarp + 1;  // warps that read an item's description
 // Tensor memory columns: O tiles, S tiles, P tiles.
+constexpr int kKeptPrompts = 512;             // kept in shared memory, further ones are read again
 constexpr uint32_t kTmemColumns = 512, kTmemS = kQTiles * kTile, kTmemP = kTmemS + kQTiles * kKeys;
 static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "tensor memory is full");
 // Registers of the softmax warps, of the result warps and of the rest: 256 x 184
@@ -81,6 +82,7 @@ struct PromptSmem {
   __align__(1024) uint8_t v[kStages][kKeyTileBytes];
   float sum[kQTiles][kTile];  // of the probabilities of each row
   Item item[2];
+  int2 prompts[kKeptPrompts];  // first row and rows of the first prompts
   __align__(16) uint8_t block[16];  // answer to the request for a block
   __align__(8) uint64_t block_full;
   uint64_t item_full[2], item_empty[2];
@@ -237,70 +239,57 @@ __device__ __forceinline__ void commit(uint64_t* bar, bool wanted = true) {
 // Items.  An item is a pair of query tiles of some prompt and a KV head; pair i
 // of a prompt costs the more the larger i is, and the same in every prompt.
 
-// A prompt as a lane has it, in groups of 32: the first kKept groups stay in
-// registers, further ones are read again whenever they are asked for.
-struct Prompt {
-  int row0, length, pairs;
-};
-constexpr int kKept = 4;
-
-__device__ __forceinline__ Prompt load_prompt(const PromptParams& p, int r) {
-  Prompt x{0, 0, 0};
-  if (r < p.prompts) {
-    x.row0 = max(0, min(p.starts[r], p.tokens));
-    x.length = max(0, min(p.starts[r + 1], p.tokens) - x.row0);
-  }
-  x.pairs = (x.length + (kQTiles * kTile >> p.group_log2) - 1) >> (8 - p.group_log2);
-  return x;
-}
-
 // Finds items by their number, one warp.  They are numbered in the order "all
 // prompts' pairs i, from the largest i down" (for every KV head), so that the
-// longest are under way first; the warp walks down the levels i (numbers must
-// not fall from call to call), and `above` counts the pairs of the levels done.
+// longest are under way first; the warp walks down the levels i, and within one
+// through the prompts, so numbers must not fall from call to call.
 struct ItemPicker {
   const PromptParams& p;
+  PromptSmem& sm;
   const int lane;
-  Prompt kept[kKept];
   int level = -1;
-  uint32_t above = 0, here = 0;  // `here`: prompts that have a pair of this level
+  uint32_t above = 0, here = 0;    // pairs of the levels done; prompts that have one of this level
+  int group = 0;                   // prompts 32 group .. are next,
+  uint32_t before = 0;             // and so many before them have a pair of this level
 
-  // f(group of 32 prompts) in order, until it returns true (f is warp-uniform).
-  template <typename F>
-  __device__ __forceinline__ void each_group(F&& f) {
-#pragma unroll
-    for (int g = 0; g < kKept; ++g) {
-      if (32 * g >= p.prompts) return;
-      if (f(kept[g])) return;
+  __device__ __forceinline__ int2 read_prompt(int r) const {  // first row and rows
+    int2 x = make_int2(0, 0);
+    if (r < p.prompts) {
+      x.x = max(0, min(p.starts[r], p.tokens));
+      x.y = max(0, min(p.starts[r + 1], p.tokens) - x.x);
     }
-#pragma unroll 1
-    for (int r = 32 * kKept; r < p.prompts; r += 32)
-      if (f(load_prompt(p, r + lane))) return;
+    return x;
   }
-  __device__ __forceinline__ void count_level() {
+  __device__ __forceinline__ int2 prompt(int r) const { return r < kKeptPrompts ? sm.prompts[r] : read_prompt(r); }
+  __device__ __forceinline__ int pairs(int rows) const {
+    return (rows + (kQTiles * kTile >> p.group_log2) - 1) >> (8 - p.group_log2);
+  }
+  __device__ __forceinline__ bool reaches(int r) const { return pairs(prompt(r).y) > level; }
+
+  __device__ __forceinline__ void enter_level() {
     here = 0;
-    each_group([&](const Prompt& x) {
-      here += (uint32_t)__popc(__ballot_sync(0xffffffffu, x.pairs > level));
-      return false;
-    });
+    group = 0;
+    before = 0;
+    for (int r = 0; r < p.prompts; r += 32) here += (uint32_t)__popc(__ballot_sync(0xffffffffu, reaches(r + lane)));
   }
-  __device__ __forceinline__ ItemPicker(const PromptParams& params, int lane_) : p(params), lane(lane_) {
-#pragma unroll
-    for (int g = 0; g < kKept; ++g) kept[g] = load_prompt(p, 32 * g + lane);
-    uint32_t most = 0;
-    each_group([&](const Prompt& x) {
-      most = max(most, __reduce_max_sync(0xffffffffu, (unsigned)x.pairs));
-      return false;
-    });
-    level = (int)most - 1;
-    if (level >= 0) count_level();
+  __device__ __forceinline__ ItemPicker(const PromptParams& params, PromptSmem& smem, int lane_)
+      : p(params), sm(smem), lane(lane_) {
+    int most = 0;
+    for (int r = lane; r < (p.prompts + 31 & ~31); r += 32) {
+      const int2 x = read_prompt(r);
+      if (r < kKeptPrompts) sm.prompts[r] = x;
+      most = max(most, pairs(x.y));
+    }
+    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
+    __syncwarp();
+    if (level >= 0) enter_level();
   }
   // Item number `at`; head -1: there are fewer.
   __device__ __forceinline__ Item item(uint32_t at) {
     const uint32_t x = at / (uint32_t)p.kv_heads;  // pair of every head
     while (level >= 0 && x >= above + here) {
       above += here;
-      if (--level >= 0) count_level();
+      if (--level >= 0) enter_level();
     }
     const int tile_tokens = kTile >> p.group_log2;
     Item w;
@@ -310,20 +299,20 @@ struct ItemPicker {
     w.last[0] = w.last[1] = -1;
     if (level < 0) return w;
     w.head = (int)(at % (uint32_t)p.kv_heads);
-    int rank = (int)(x - above);
-    each_group([&](const Prompt& of) {
-      uint32_t have = __ballot_sync(0xffffffffu, of.pairs > level);
-      const int count = __popc(have);
-      if (rank >= count) {
-        rank -= count;
-        return false;
+    const uint32_t rank = x - above;  // of the prompts of this level
+    for (; 32 * group < p.prompts; ++group) {
+      const int2 mine = prompt(32 * group + lane);
+      uint32_t have = __ballot_sync(0xffffffffu, pairs(mine.y) > level);
+      if (rank >= before + (uint32_t)__popc(have)) {
+        before += (uint32_t)__popc(have);
+        continue;
       }
-      for (; rank > 0; --rank) have &= have - 1;
+      for (uint32_t skip = rank - before; skip > 0; --skip) have &= have - 1;
       const int src = __ffs(have) - 1;
-      w.row0 = __shfl_sync(0xffffffffu, of.row0, src);
-      w.length = __shfl_sync(0xffffffffu, of.length, src);
-      return true;
-    });
+      w.row0 = __shfl_sync(0xffffffffu, mine.x, src);
+      w.length = __shfl_sync(0xffffffffu, mine.y, src);
+      break;
+    }
 #pragma unroll
     for (int t = 0; t < kQTiles; ++t) {
       const int t0 = w.tok0 + t * tile_tokens;
@@ -365,7 +354,7 @@ __device__ __forceinline__ bool block_taken(PromptSmem& sm, uint32_t& number) {
 }
 
 __device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& sm, int lane) {
-  ItemPicker picker(p, lane);
+  ItemPicker picker(p, sm, lane);
   uint32_t number = blockIdx.x, asked = 0;
   bool more = true, answered = true;  // `number` is a block of this CTA's
   for (int n = 0;; ++n) {

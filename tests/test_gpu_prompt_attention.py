@@ -66,7 +66,7 @@ def _starts(lens):
 
 LENS = [
     [1], [2], [127], [128], [129], [255], [256], [257], [1, 1, 1], [0, 5, 0, 0, 130, 0], [33, 1, 200, 16, 15, 17],
-    [700, 3, 1025], [1] * 70, [64] * 40 + [0] * 40 + [3],
+    [700, 3, 1025], [1] * 70, [64] * 40 + [0] * 40 + [3], [2, 0, 1] * 200 + [300, 7],
 ]
 
 

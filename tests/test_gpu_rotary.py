@@ -151,6 +151,19 @@ def test_unrotated_dims_keep_their_bits_and_rows_stay_apart() -> None:
     assert bad[7, 2] and int(bad.sum()) == 1 and not torch.isnan(k_out).any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_at_any_address(dtype) -> None:
+    """A weight that is a slice of a larger tensor: only its own alignment is asked for."""
+    _, q, k, _ = _heads(20, 3, 2)
+    rotary, positions = make_rotary(q.device), torch.arange(20, device="cuda")
+    freq, factor = rotary_frequencies()
+    weights = torch.rand(2 * DIM + 1, device="cuda").to(dtype)[1:]
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    norm_rotary(q, k, positions, rotary, q_out, k_out, weights[:DIM], weights[DIM:])
+    _check(q_out, _reference(q, weights[:DIM], positions, freq, factor, 128, False))
+    _check(k_out, _reference(k, weights[DIM:], positions, freq, factor, 128, False))
+
+
 def test_rows_of_zeros_and_of_large_and_small_values() -> None:
     q = torch.zeros(3, 2, DIM, dtype=torch.bfloat16, device="cuda")
     q[1], q[2] = 1e18, 1e-18
