@@ -654,8 +654,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
       float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
       // The reference follows the running maximum once that is kRescaleSlack above it.
       if (__any_sync(0xffffffffu, j == 0 || !(tile_max <= ref + kRescaleSlack))) {
-        // An infinite or NaN maximum makes the whole row NaN (its output is then
-        // computed again, key by key).
+        // An infinite or NaN maximum makes the whole row NaN.
         if (!(tile_max < INFINITY)) tile_max = NAN;
         if (j == 0) {
           ref = tile_max == -INFINITY ? 0.f : tile_max;
@@ -717,37 +716,69 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
 // ---------------------------------------------------------------------------
 // Results.
 
-// One query row by one warp, key by key over the keys that it sees, lane l
-// carrying dims 4 l .. 4 l + 3.  The tensor cores also multiply the values of
+// One query row by one warp over the keys that it sees, kRowKeys at a time, lane
+// l carrying dims 4 l .. 4 l + 3.  The tensor cores also multiply the values of
 // later tokens (by zero probabilities), so a row that came out NaN or infinite
-// is computed again here: what it then shows is its own.
+// from a sound sum is computed again here: what it then shows is its own.  Its
+// weights are 2^-kRowShift smaller, so that no sum of finite values overflows.
+constexpr int kRowKeys = 8;
+constexpr float kRowShift = 32.f;  // tokens are fewer than 2^30
+
 __device__ __forceinline__ void prompt_row(const PromptParams& p, int row0, int tok, int kv_head, int q_head, int lane) {
-  const auto load = [&](const Heads& h, int row, int head, float (&x)[4]) {
-    const uint2 two = *reinterpret_cast<const uint2*>(h.at + row * h.token + head * h.head + 4 * lane);
+  const auto load = [&](const Heads& h, int row, int head) {
+    return *reinterpret_cast<const uint2*>(h.at + row * h.token + head * h.head + 4 * lane);
+  };
+  const auto widen = [](uint2 two, float (&x)[4]) {
     x[0] = __uint_as_float(two.x << 16);
     x[1] = __uint_as_float(two.x & 0xffff0000u);
     x[2] = __uint_as_float(two.y << 16);
     x[3] = __uint_as_float(two.y & 0xffff0000u);
   };
-  float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-  load(p.q, row0 + tok, q_head, q);
+  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+  widen(load(p.q, row0 + tok, q_head), q);
 #pragma unroll 1
-  for (int j = 0; j <= tok; ++j) {
-    load(p.k, row0 + j, kv_head, k);
-    load(p.v, row0 + j, kv_head, v);
-    float score = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+  for (int j0 = 0; j0 <= tok; j0 += kRowKeys) {
+    uint2 keys[kRowKeys], values[kRowKeys];
+    float score[kRowKeys], new_top = top;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) score += __shfl_xor_sync(0xffffffffu, score, d);
-    score *= p.scale_log2;
-    const float new_top = fmaxf(top, score), ref = new_top == -INFINITY ? 0.f : new_top;
-    const float keep = ex2(top - ref), weight = ex2(score - ref);
-    sum = sum * keep + weight;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (new_top > top) o[x] *= keep;
-      if (weight != 0.f) o[x] += weight * v[x];  // also for NaN
+    for (int u = 0; u < kRowKeys; ++u) {
+      const int row = row0 + min(j0 + u, tok);
+      keys[u] = load(p.k, row, kv_head);
+      values[u] = load(p.v, row, kv_head);
     }
-    top = new_top;
+#pragma unroll
+    for (int u = 0; u < kRowKeys; ++u) {
+      float k[4];
+      widen(keys[u], k);
+      score[u] = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+      for (int u = 0; u < kRowKeys; ++u) score[u] += __shfl_xor_sync(0xffffffffu, score[u], d);
+#pragma unroll
+    for (int u = 0; u < kRowKeys; ++u) {
+      score[u] = j0 + u <= tok ? score[u] * p.scale_log2 : -INFINITY;
+      new_top = fmaxf(new_top, score[u]);
+    }
+    const float ref = new_top == -INFINITY ? 0.f : new_top;
+    if (new_top > top) {
+      const float keep = ex2(top - ref);
+      sum *= keep;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[x] *= keep;
+      top = new_top;
+    }
+#pragma unroll
+    for (int u = 0; u < kRowKeys; ++u) {
+      const float weight = ex2(score[u] - ref - kRowShift);
+      float v[4];
+      widen(values[u], v);
+      sum += weight;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (weight != 0.f) o[x] += weight * v[x];  // also for NaN
+    }
   }
   const float inv = sum > 0.f ? 1.f / sum : sum;
   *reinterpret_cast<uint2*>(p.out + (row0 + tok) * p.o_token + q_head * p.o_head + 4 * lane) =
@@ -818,7 +849,9 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
       }
       float a, b;
       unpack2(stray, a, b);
-      const bool finite = (a == 0.f && b == 0.f) || w.tok0 + ((t * kTile + row) >> p.group_log2) >= w.length;
+      // A NaN among the scores that a row sees makes its sum NaN, and the row with it.
+      const bool finite =
+          (a == 0.f && b == 0.f) || sum != sum || w.tok0 + ((t * kTile + row) >> p.group_log2) >= w.length;
       __syncwarp();
       for (uint32_t again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
         const int r = first_row + __ffs(again) - 1;

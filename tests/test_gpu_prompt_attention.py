@@ -143,6 +143,32 @@ def test_value_infinities_show_where_they_are_seen() -> None:
     assert bool(torch.isfinite(out[..., rest]).all())
 
 
+@pytest.mark.parametrize("group", [1, 8])
+def test_values_whose_weighted_sum_passes_the_range(group) -> None:
+    """Equal weights over 1e38: the result is 1e38, though the sum of the values is not in range."""
+    n = 700
+    q, k, v = _inputs(n, 2, group, seed=12)
+    q[:] = 0.0
+    v[:] = 1e38
+    v[:, 1, 3] = -1e38
+    out = torch.zeros(n, 2 * group, DIM, dtype=torch.bfloat16, device="cuda")
+    prompt_attention(q, k, v, _starts([n]), SCALE, out)
+    # One rounding to BF16, and 2^-24 for each of at most 700 terms of a sum in FP32.
+    want = v.repeat_interleave(group, 1).double()
+    assert float(((out.double() - want) / want).abs().max()) <= 2.0**-8 + 700 * 2.0**-24
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "v inf"])
+def test_prompts_of_nothing_but_nan_and_infinities(where) -> None:
+    """A step that a broken layer left without a number: the result says so, in the time of a sound one."""
+    lens = [4000, 1, 333]
+    q, k, v = _inputs(sum(lens), 4, 4, seed=13)
+    {"q": q, "k": k, "v": v, "v inf": v}[where].fill_(float("inf") if where == "v inf" else float("nan"))
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    assert bool((out == float("inf")).all() if where == "v inf" else torch.isnan(out).all())
+
+
 def test_single_tokens_return_their_values() -> None:
     q, k, v = _inputs(9, 3, 8)
     out = torch.empty(9, 24, DIM, dtype=torch.bfloat16, device="cuda")
