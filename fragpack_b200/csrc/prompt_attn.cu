@@ -75,6 +75,12 @@ struct Item {
   int last[kQTiles];       // last key tile of each query tile; -1: it has no rows
 };
 
+// A wait that ran out raises `abort`, and every later one gives up at once.
+struct PromptWait {
+  volatile int abort;
+  uint32_t limit;  // cycles
+};
+
 struct PromptSmem {
   __align__(1024) uint8_t q[kQTiles][kTileBytes];
   __align__(1024) uint8_t o[kTileBytes];  // results on their way out
@@ -95,7 +101,7 @@ struct PromptSmem {
   uint64_t o_done[kQTiles], o_free[kQTiles];          // the item's last O product done; O read
   uint64_t drained[2];
   uint32_t tmem_base;
-  WaitState wait;
+  PromptWait wait;
 };
 
 // BF16 [tokens, heads, 128], strides in scalars.
@@ -113,9 +119,15 @@ struct PromptParams {
   int prompts, tokens, kv_heads;
   int group, group_log2;
   float scale_log2;
-  long long wait_limit;
+  uint32_t wait_limit;
   int skip_tile;  // test hook: this K tile of an item is not loaded (-1: none)
 };
+
+__device__ __forceinline__ uint32_t clock32() {
+  uint32_t c;
+  asm volatile("mov.u32 %0, %clock;" : "=r"(c));
+  return c;
+}
 
 // As bounded_wait, inlined whole (a call would keep the register split from
 // taking effect) and without a suspend-time hint: with hints of 2 and 20
@@ -129,18 +141,15 @@ __device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, WaitState* ws) {
+// What runs out is reported once, at the end of the kernel.
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, PromptWait* ws) {
   if (arrived(bar, parity)) return true;
-  volatile int* abort = &ws->abort;
-  const long long t0 = clock64();
+  const uint32_t t0 = clock32();
 #pragma unroll 1
-  while (!arrived(bar, parity)) {
-    if (*abort) return false;
-    if (clock64() - t0 > ws->limit) {
-      *abort = 1;
-      atomicOr(ws->status, FP_DECODE_WAIT_TIMEOUT);
-    }
-  }
+  do {
+    if (ws->abort) return false;
+    if (clock32() - t0 > ws->limit) ws->abort = 1;
+  } while (!arrived(bar, parity));
   return true;
 }
 
@@ -280,9 +289,8 @@ struct ItemPicker {
       if (r < kKeptPrompts) sm.prompts[r] = x;
       most = max(most, pairs(x.y));
     }
-    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
+    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);  // above every pair
     __syncwarp();
-    if (level >= 0) enter_level();
   }
   // Item number `at`; head -1: there are fewer.
   __device__ __forceinline__ Item item(uint32_t at) {
@@ -433,7 +441,7 @@ __device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& s
     }
     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
   }
-  if (lane != 0 || !*(volatile int*)&sm.wait.abort) return;
+  if (lane != 0 || !sm.wait.abort) return;
   // A wait ran out somewhere.  Shared memory is given back at the end of the
   // kernel, so this thread stays until its own copies have landed (bounded: a
   // tile that was left out never lands).
@@ -721,7 +729,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
 // later tokens (by zero probabilities), so a row that came out NaN or infinite
 // from a sound sum is computed again here: what it then shows is its own.  Its
 // weights are 2^-kRowShift smaller, so that no sum of finite values overflows.
-constexpr int kRowKeys = 8;
+constexpr int kRowKeys = 2;
 constexpr float kRowShift = 32.f;  // tokens are fewer than 2^30
 
 __device__ __forceinline__ void prompt_row(const PromptParams& p, int row0, int tok, int kv_head, int q_head, int lane) {
@@ -789,17 +797,17 @@ __device__ __forceinline__ void prompt_row(const PromptParams& p, int row0, int 
 __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int row) {
   const int lane = row & 31;
   const uint32_t tmem_o = tmem + ((uint32_t)(row & ~31) << 16);
-  uint32_t used[kQTiles] = {0, 0};
+  uint32_t used = 0;  // bit t: parity of tile t's uses
   Item w;
   for (int n = 0; next_item(sm, n, lane, w); ++n) {
-#pragma unroll
+#pragma unroll 1
     for (int t = 0; t < kQTiles; ++t) {
-      if (w.last[t] < 0) continue;
-      await(&sm.sum_full[t], used[t] & 1u, &sm.wait);
+      if ((t == 0 ? w.last[0] : w.last[1]) < 0) continue;
+      await(&sm.sum_full[t], (used >> t) & 1u, &sm.wait);
       const float sum = sm.sum[t][row];
       arrive_warp(&sm.sum_empty[t], lane);
-      await(&sm.o_done[t], used[t] & 1u, &sm.wait);
-      ++used[t];
+      await(&sm.o_done[t], (used >> t) & 1u, &sm.wait);
+      used ^= 1u << t;
       tmem_acquire();
       const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays NaN
       // Rows go out through shared memory, so that they leave in whole lines; a
@@ -898,7 +906,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     mbar_init(&sm.drained[0], 1);
     mbar_init(&sm.drained[1], 1);
     sm.wait.abort = 0;
-    sm.wait.status = &g_prompt_status;
     sm.wait.limit = p.wait_limit;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -932,6 +939,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
   }
   tmem_release();
   __syncthreads();
+  if (tid == 0 && sm.wait.abort) atomicOr(&g_prompt_status, FP_DECODE_WAIT_TIMEOUT);
   if (warp == 0) {
     tmem_acquire();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
@@ -1029,7 +1037,7 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.group = group;
   p.group_log2 = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.wait_limit = wait_debug().limit;
+  p.wait_limit = (uint32_t)std::min<long long>(wait_debug().limit, 0xf0000000LL);
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
   // Every prompt has at most one pair of tiles that is not full.
   const int64_t items = (tokens / (kQTiles * tile_tokens) + prompts) * kv_heads;
