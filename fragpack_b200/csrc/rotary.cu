@@ -256,10 +256,13 @@ __global__ void __launch_bounds__(kRowThreads, kRows == 4 ? 4 : 1) rotary_rows_k
 // normed and rotated into shared memory and leaves in 16-byte pieces of whole
 // lines.  Tokens outside every such group go to their places one by one, by the
 // CTA that has them among its sixteen.
-constexpr int kKvSlice = 4, kQuerySlice = 16;
+// Slices of eight query heads against sixteen, 32 + 8 heads: prompts of 512 tokens
+// 5.7 / 8.0 us, of 1,000 tokens 6.9 / 8.5 us, of 8,192 tokens 44.8 / 45.1 us; with
+// four, two prompts of 8,192 tokens (32 + 32 heads) take 176 us against 164.
+constexpr int kKvSlice = 4, kQuerySlice = 8;
 // Up to here rotary_rows_kernel.  Rows against groups: 256 decode tokens (64 + 8
-// heads) 8.0 / 9.6 us, 512 of them 14.6 / 12.3 us; one prompt of 256 tokens (32 +
-// 8 heads) 4.3 / 5.9 us, of 400 tokens 6.1 / 5.9 us.  Two prompts of 8,192 tokens
+// heads) 7.8 / 9.6 us, 512 of them 14.9 / 12.3 us; one prompt of 256 tokens (32 +
+// 8 heads) 4.2 / 5.1 us, of 400 tokens 6.4 / 5.8 us.  Two prompts of 8,192 tokens
 // with 32 + 32 heads: 418 / 164 us, 0.89 of the measured copy bandwidth.
 constexpr int kFewTokens = 384;
 constexpr int kTileRow = 272;  // bytes of a staged token row (256 + pad)
