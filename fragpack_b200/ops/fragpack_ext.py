@@ -14,6 +14,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -77,7 +78,7 @@ class FpRotary(ctypes.Structure):
 
 
 class FpHeads(ctypes.Structure):
-    """``fp_heads`` of ``include/fragpack_b200.h``."""
+    """``fp_heads`` of ``include/fragpack_b200.h`` (see :data:`pack_heads`)."""
 
     _fields_ = [
         ("input", c_ptr),
@@ -89,6 +90,10 @@ class FpHeads(ctypes.Structure):
         ("heads", c_i32),
     ]
 
+
+# An FpHeads' bytes from its fields, passed in place of a pointer to one: a third
+# of the time that the structure takes to build.
+pack_heads = struct.Struct("PPqqqqi4x").pack
 
 # name -> argument types; every function returns int.
 _SIGNATURES = {
@@ -166,9 +171,14 @@ def require_cuda(tensor: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} must be a CUDA tensor: fragpack_b200.ops has no CPU fallback")
 
 
+# torch.cuda.current_device without its look at whether CUDA is initialised: who
+# has a CUDA tensor has initialised it.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def on_device(device: int) -> contextlib.AbstractContextManager:
     """Make CUDA device ``device`` current for a launch, if it is not already."""
-    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device == _current_device() else torch.cuda.device(device)
 
 
 # Without the Stream object (3 us of host time a call) where torch has such a getter.
@@ -178,7 +188,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def stream_ptr() -> int:
     """Handle of the current CUDA stream."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -190,6 +200,7 @@ __all__ = [
     "check",
     "extension",
     "on_device",
+    "pack_heads",
     "require_cuda",
     "stream_ptr",
 ]

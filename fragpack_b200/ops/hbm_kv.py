@@ -387,7 +387,7 @@ class HbmKvStore:
         k = head_set("key", key, key_out, tokens, device)
         v_stride = value.stride()
         if (
-            k.heads != self.kv_heads
+            key.shape[1] != self.kv_heads
             or value.shape != key.shape
             or v_stride[2] != 1
             or value.dtype is not torch.bfloat16
@@ -407,7 +407,7 @@ class HbmKvStore:
         with on_device(device):
             check(
                 extension().fp_hbm_append(
-                    self._store_ref, ctypes.byref(q), ctypes.byref(k), value.data_ptr(), v_stride[0], v_stride[1],
+                    self._store_ref, q, k, value.data_ptr(), v_stride[0], v_stride[1],
                     *operands, slot_mapping.data_ptr(), tokens, rotary._ref, eps, layer, stream_ptr(),
                 )
             )

@@ -24,11 +24,11 @@ import numpy as np
 import torch
 
 from fragpack_b200.ops.fragpack_ext import (
-    FpHeads,
     FpRotary,
     check,
     extension,
     on_device,
+    pack_heads,
     require_cuda,
     stream_ptr,
 )
@@ -169,8 +169,8 @@ _BF16, _FP32, _INT64, _INT32 = torch.bfloat16, torch.float32, torch.int64, torch
 
 # These checks are most of a small call's host time, so the sound case takes one
 # comparison each and the messages are found afterwards.
-def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: int) -> FpHeads:
-    """Check one set of heads and its result on CUDA device ``device`` and describe them to the library."""
+def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: int, device: int) -> bytes:
+    """Check one set of heads and its result on CUDA device ``device``; returns the ``fp_heads`` that describes them."""
     shape, stride = heads.shape, heads.stride()
     if (
         len(shape) != 3
@@ -185,14 +185,14 @@ def head_set(name: str, heads: torch.Tensor, out: torch.Tensor | None, tokens: i
             f"not {heads.dtype} {tuple(shape)} on {heads.device} with strides {stride}"
         )
     if out is None:
-        return FpHeads(heads.data_ptr(), None, stride[0], stride[1], 0, 0, shape[1])
+        return pack_heads(heads.data_ptr(), 0, stride[0], stride[1], 0, 0, shape[1])
     to = out.stride()
     if out.shape != shape or to[2] != 1 or out.dtype is not _BF16 or out.get_device() != device:
         raise RuntimeError(
             f"{name}_out must be bfloat16 {tuple(shape)} on cuda:{device} with a contiguous head dim, "
             f"not {out.dtype} {tuple(out.shape)} on {out.device} with strides {to}"
         )
-    return FpHeads(heads.data_ptr(), out.data_ptr(), stride[0], stride[1], to[0], to[1], shape[1])
+    return pack_heads(heads.data_ptr(), out.data_ptr(), stride[0], stride[1], to[0], to[1], shape[1])
 
 
 def rotary_operands(
@@ -246,7 +246,7 @@ def _weight(weight: torch.Tensor, dtype: torch.dtype, device: int) -> int:
     return weight.data_ptr()
 
 
-_NO_HEADS = FpHeads(None, None, 0, 0, 0, 0, 0)
+_NO_HEADS = pack_heads(0, 0, 0, 0, 0, 0, 0)
 
 
 def norm_rotary(
@@ -295,7 +295,7 @@ def norm_rotary(
     with on_device(device):
         check(
             extension().fp_norm_rotary(
-                byref(q), byref(k), *operands, tokens, rotary._ref, eps, stream_ptr(),
+                q, k, *operands, tokens, rotary._ref, eps, stream_ptr(),
             )
         )
 

@@ -11,7 +11,7 @@ import torch
 
 from fragpack_b200.compression.attn_tables import device_tables
 from fragpack_b200.integrations.vllm import backend
-from fragpack_b200.ops.fragpack_ext import FpHeads, FpRotary, FpStore, extension
+from fragpack_b200.ops.fragpack_ext import FpHeads, FpRotary, FpStore, extension, pack_heads
 from fragpack_b200.ops.hbm_kv import HbmKvStore, page_bytes
 from fragpack_b200.ops.prompt_attn import prompt_attention
 from fragpack_b200.ops.rotary import make_rotary, norm_rotary, rotary_frequencies
@@ -197,3 +197,9 @@ def test_run_layer_calls_the_operators_it_is_asked_for(monkeypatch, fused_append
     first = [("append", 12)] if fused_append else [("norm_rotary", 12), ("write", 12)]
     second = [("prompt", [0, 7])] if over_prompt else [("records", 7)]
     assert calls == first + second + [("records", 5), "encode", "commit"]
+
+
+def test_packed_heads_are_the_structure() -> None:
+    fields = (1 << 40, 0, 3, -4, 5, 6, 7)
+    structure = FpHeads(*fields)
+    assert ctypes.string_at(ctypes.byref(structure), ctypes.sizeof(FpHeads)) == pack_heads(*fields)
