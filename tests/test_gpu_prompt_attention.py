@@ -101,6 +101,24 @@ def test_strided_tensors(layout, h, group) -> None:
     _check(out, _reference(q, k, v, lens), 201)
 
 
+def test_tokens_far_apart() -> None:
+    """Token strides that take offsets past 32 bits, in the inputs and the result, heads redone key by key among them."""
+    lens, h, group = [17, 3, 22], 2, 2
+    q, k, v = _inputs(sum(lens), h, group, seed=8)
+    v[30, 1, 7] = float("inf")
+    heads = torch.cat([q, k, v, torch.zeros_like(q)], 1)
+    stride = (1 << 32) // (sum(lens) - 1) // 8 * 8 + 8
+    far = torch.empty((sum(lens) - 1) * stride + heads.shape[1] * DIM, dtype=torch.bfloat16, device="cuda")
+    assert far.numel() > 1 << 32
+    far = far.as_strided(heads.shape, (stride, DIM, 1))
+    far.copy_(heads)
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    at = h * group
+    prompt_attention(far[:, :at], far[:, at : at + h], far[:, at + h : at + 2 * h], _starts(lens), SCALE, far[:, at + 2 * h :])
+    assert torch.equal(far[:, at + 2 * h :], out) and bool(torch.isinf(out[30:, 2:, 7]).all())
+
+
 @pytest.mark.parametrize("group", [1, 8])
 def test_what_lies_outside_the_prompts_reaches_nothing_and_stays(group) -> None:
     """Rows before, between (clamped starts) and behind the prompts hold NaN; their outputs keep their fill."""

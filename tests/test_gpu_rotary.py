@@ -351,3 +351,35 @@ def test_rotary_frequency_period() -> None:
     norm_rotary(q, None, torch.tensor([0, 4, 1 << 20], device="cuda"), rotary, out, None)
     assert torch.equal(out[0], q[0]) and torch.equal(out[1], q[0])
     assert bool(((out[2].double() - q[0].double()).abs() <= 2.0**-8 * q[0].double().abs() + 1e-4).all())
+
+
+def _far_apart(heads, stride):
+    """The same values with tokens `stride` scalars apart, so that offsets pass 32 bits."""
+    tokens = heads.shape[0]
+    far = torch.empty((tokens - 1) * stride + heads.shape[1] * DIM, dtype=torch.bfloat16, device="cuda")
+    assert far.numel() > 1 << 32
+    far = far.as_strided(heads.shape, (stride, DIM, 1))
+    far.copy_(heads)
+    return far
+
+
+@pytest.mark.parametrize("tokens", [40, 420])
+def test_tokens_far_apart(tokens) -> None:
+    """Rows of 2^32 scalars and more, in place, alone and on the way into the store (few and many tokens)."""
+    h, group = 2, 2
+    qkv, q, k, v = _heads(tokens, h * group, h, seed=3)
+    far = _far_apart(qkv, -(-(1 << 32) // (tokens - 1) // 8) * 8 + 8)
+    positions, slots = torch.arange(tokens, device="cuda"), torch.arange(tokens, device="cuda")
+    near, wide = _store(h), _store(h)
+    rotary = make_rotary(near.counters.device)
+    for store in (near, wide):
+        store.prepare(slots, tokens, np.arange(-(-tokens // T), dtype=np.int32))
+    wide.append(0, far[:, : h * group], far[:, h * group : h * (group + 1)], far[:, h * (group + 1) :], positions, slots,
+                rotary, far[:, : h * group], far[:, h * group : h * (group + 1)])
+    near.append(0, q, k, v, positions, slots, rotary, q, k)
+    assert torch.equal(far, qkv)
+    blocks = range(-(-tokens // T))
+    assert torch.equal(_records(near, 0, blocks), _records(wide, 0, blocks))
+    norm_rotary(far[:, : h * group], None, positions, rotary, far[:, : h * group], None)
+    norm_rotary(q, None, positions, rotary, q, None)
+    assert torch.equal(far, qkv)
