@@ -76,6 +76,7 @@ constexpr int kScoreWarp = kSoftmaxWarps + kResultWarps, kValueWarp = kScoreWarp
 constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kResultWarps + 4);  // whole warpgroups
 constexpr int kItemReaders = kLoadWarp + 1;  // warps that read an item's description
 // Tensor memory columns: O tiles, S tiles, P tiles.
+constexpr int64_t kChunkBytes = 64 << 20;     // see head_chunk
 constexpr int kKeptPrompts = 512;             // kept in shared memory, further ones are read again
 constexpr uint32_t kTmemColumns = 512, kTmemS = kQTiles * kTile, kTmemP = kTmemS + kQTiles * kKeys;
 static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "tensor memory is full");
@@ -143,6 +144,7 @@ struct PromptParams {
   int64_t o_token, o_head;
   const int32_t* starts;
   int prompts, tokens, kv_heads;
+  int head_chunk;  // KV heads whose items come before the next ones'
   int group, group_log2;
   float scale_log2;
   uint32_t wait_limit;
@@ -274,15 +276,17 @@ __device__ __forceinline__ void commit(uint64_t* bar, bool wanted = true) {
 // Items.  An item is a pair of query tiles of some prompt and a KV head; pair i
 // of a prompt costs the more the larger i is, and the same in every prompt.
 
-// Finds items by their number, one warp.  They are numbered in the order "all
-// prompts' pairs i, from the largest i down" (for every KV head), so that the
-// longest are under way first; the warp walks down the levels i, and within one
-// through the prompts, so numbers must not fall from call to call.
+// Finds items by their number, one warp.  They are numbered head_chunk KV heads
+// after head_chunk KV heads and within those in the order "all prompts' pairs i,
+// from the largest i down", so that the longest are under way first; the warp
+// walks down the levels i, and within one through the prompts, so numbers must
+// not fall from call to call.
 struct ItemPicker {
   const PromptParams& p;
   PromptSmem& sm;
   const int lane;
-  int level = -1;
+  int levels, level = -1;
+  uint32_t total = 0, chunk = 0;   // pairs of all prompts; the chunk of heads that the walk is in
   uint32_t above = 0, here = 0;    // pairs of the levels done; prompts that have one of this level
   int group = 0;                   // prompts 32 group .. are next,
   uint32_t before = 0;             // and so many before them have a pair of this level
@@ -309,18 +313,29 @@ struct ItemPicker {
   }
   __device__ __forceinline__ ItemPicker(const PromptParams& params, PromptSmem& smem, int lane_)
       : p(params), sm(smem), lane(lane_) {
-    int most = 0;
+    int most = 0, sum = 0;
     for (int r = lane; r < (p.prompts + 31 & ~31); r += 32) {
       const int2 x = read_prompt(r);
       if (r < kKeptPrompts) sm.prompts[r] = x;
       most = max(most, pairs(x.y));
+      sum += pairs(x.y);
     }
-    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);  // above every pair
+    levels = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+    total = __reduce_add_sync(0xffffffffu, (unsigned)sum);
+    level = levels;  // above every pair
     __syncwarp();
   }
   // Item number `at`; head -1: there are fewer.
   __device__ __forceinline__ Item item(uint32_t at) {
-    const uint32_t x = at / (uint32_t)p.kv_heads;  // pair of every head
+    const uint32_t in_chunk = max(total * (uint32_t)p.head_chunk, 1u), next = at / in_chunk;
+    if (next != chunk) {
+      chunk = next;
+      level = levels;
+      above = here = 0;
+    }
+    const int head0 = (int)chunk * p.head_chunk, heads = min(p.head_chunk, p.kv_heads - head0);
+    if (heads <= 0) level = -1;
+    const uint32_t y = at - chunk * in_chunk, x = y / (uint32_t)max(heads, 1);  // pair of every head of the chunk
     while (level >= 0 && x >= above + here) {
       above += here;
       if (--level >= 0) enter_level();
@@ -332,7 +347,7 @@ struct ItemPicker {
     w.tok0 = max(level, 0) * kQTiles * tile_tokens;
     w.last[0] = w.last[1] = -1;
     if (level < 0) return w;
-    w.head = (int)(at % (uint32_t)p.kv_heads);
+    w.head = head0 + (int)(y - x * (uint32_t)heads);
     const uint32_t rank = x - above;  // of the prompts of this level
     for (; 32 * group < p.prompts; ++group) {
       const int2 mine = prompt(32 * group + lane);
@@ -1024,6 +1039,17 @@ int head_map(CUtensorMap& map, const char* name, const void* base, int64_t token
   return FP_OK;
 }
 
+// KV heads whose keys and values (512 bytes a token) are walked together: as many
+// as kChunkBytes hold, so that they stay in L2 while every pair of query tiles
+// reads them; rather fewer than chunks of different sizes, whose last one would
+// leave SMs without work.
+int head_chunk(int64_t tokens, int kv_heads) {
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kv_heads, kChunkBytes / (tokens * 512)));
+  for (int n = most; 2 * n > most; --n)
+    if (kv_heads % n == 0) return n;
+  return most;
+}
+
 bool strides_fit(const void* base, int64_t tokens, int64_t heads, int64_t token_stride, int64_t head_stride) {
   const auto fits = [](int64_t n, int64_t stride) {
     return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38));
@@ -1071,6 +1097,7 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.prompts = prompts;
   p.tokens = (int)tokens;
   p.kv_heads = kv_heads;
+  p.head_chunk = head_chunk(tokens, kv_heads);
   p.group = group;
   p.group_log2 = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
   p.scale_log2 = scale * 1.4426950408889634f;
