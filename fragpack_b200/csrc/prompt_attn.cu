@@ -118,7 +118,7 @@ struct PromptSmem {
   int2 prompts[kKeptPrompts];  // first row and rows of the first prompts
   __align__(16) uint8_t block[16];  // answer to the request for a block
   __align__(8) uint64_t block_full;
-  uint64_t item_full[2], item_empty[2];
+  uint64_t item_full[2], item_empty[2], item_wanted;
   uint64_t q_full[kQTiles], q_empty[kQTiles];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_ready[kQTiles], s_free[kQTiles];         // S product done; S read
@@ -286,7 +286,8 @@ struct ItemPicker {
   PromptSmem& sm;
   const int lane;
   int levels, level = -1;
-  uint32_t total = 0, chunk = 0;   // pairs of all prompts; the chunk of heads that the walk is in
+  uint32_t in_chunk = 0, first = 0;  // items of a chunk of heads; number of the first one of the present chunk
+  int head0 = 0;                   // its first head
   uint32_t above = 0, here = 0;    // pairs of the levels done; prompts that have one of this level
   int group = 0;                   // prompts 32 group .. are next,
   uint32_t before = 0;             // and so many before them have a pair of this level
@@ -321,21 +322,20 @@ struct ItemPicker {
       sum += pairs(x.y);
     }
     levels = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
-    total = __reduce_add_sync(0xffffffffu, (unsigned)sum);
+    in_chunk = __reduce_add_sync(0xffffffffu, (unsigned)sum) * (uint32_t)p.head_chunk;
     level = levels;  // above every pair
     __syncwarp();
   }
   // Item number `at`; head -1: there are fewer.
   __device__ __forceinline__ Item item(uint32_t at) {
-    const uint32_t in_chunk = max(total * (uint32_t)p.head_chunk, 1u), next = at / in_chunk;
-    if (next != chunk) {
-      chunk = next;
-      level = levels;
+    while (head0 < p.kv_heads && at - first >= in_chunk) {
+      first += in_chunk;
+      head0 += p.head_chunk;
+      level = head0 < p.kv_heads ? levels : -1;
       above = here = 0;
     }
-    const int head0 = (int)chunk * p.head_chunk, heads = min(p.head_chunk, p.kv_heads - head0);
-    if (heads <= 0) level = -1;
-    const uint32_t y = at - chunk * in_chunk, x = y / (uint32_t)max(heads, 1);  // pair of every head of the chunk
+    const uint32_t heads = (uint32_t)max(1, min(p.head_chunk, p.kv_heads - head0));
+    const uint32_t x = (at - first) / heads;  // pair of every head of the chunk
     while (level >= 0 && x >= above + here) {
       above += here;
       if (--level >= 0) enter_level();
@@ -347,7 +347,7 @@ struct ItemPicker {
     w.tok0 = max(level, 0) * kQTiles * tile_tokens;
     w.last[0] = w.last[1] = -1;
     if (level < 0) return w;
-    w.head = head0 + (int)(y - x * (uint32_t)heads);
+    w.head = head0 + (int)(at - first - x * heads);
     const uint32_t rank = x - above;  // of the prompts of this level
     for (; 32 * group < p.prompts; ++group) {
       const int2 mine = prompt(32 * group + lane);
@@ -373,9 +373,11 @@ struct ItemPicker {
 
 // Every item has a block of the grid.  A CTA does its own and then takes over
 // blocks that have not started yet (cluster launch control), in their order, so
-// that whoever is done first goes on first.  The next block is asked for once
-// the item before the last one taken is on its way out: asked for earlier, it
-// would be bound to a CTA that may be late.
+// that whoever is done first goes on first.  The next block is asked for once the
+// load warp has begun with the last one taken and the result warps with the one
+// before: asked for earlier, it would be bound to a CTA that may be late (two
+// prompts of 8,192 tokens, 32 + 32 heads: 930 us without the wait for the load
+// warp, 899 with it; without a pause 1,051 / 1,029).
 __device__ __forceinline__ void ask_for_block(PromptSmem& sm, int lane) {
   if (lane == 0) {
     mbar_expect_tx(&sm.block_full, 16);
@@ -410,6 +412,7 @@ __device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& 
     const int slot = n & 1;
     if (n >= 2 && !await(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) break;
     if (n > 0) {
+      if (!await(&sm.item_wanted, (uint32_t)(n - 1) & 1u, &sm.wait)) break;
       ask_for_block(sm, lane);
       answered = await(&sm.block_full, asked++ & 1u, &sm.wait);
       if (!answered) break;
@@ -459,6 +462,7 @@ __device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& s
   for (int n = 0; ok && next_item(sm, n, lane, w); ++n) {
     const int last_any = max(w.last[0], w.last[1]);
     if (lane == 0) {
+      mbar_arrive(&sm.item_wanted);
       const auto load_q = [&](int t) {
         if (!ok || w.last[t] < 0) return;
         uint64_t* const full = &sm.q_full[t];
@@ -954,6 +958,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
       mbar_init(&sm.o_done[t], 1);
       mbar_init(&sm.o_free[t], kResultWarps);
     }
+    mbar_init(&sm.item_wanted, 1);
     mbar_init(&sm.block_full, 1);
     mbar_init(&sm.drained[0], 1);
     mbar_init(&sm.drained[1], 1);
@@ -1042,7 +1047,10 @@ int head_map(CUtensorMap& map, const char* name, const void* base, int64_t token
 // KV heads whose keys and values (512 bytes a token) are walked together: as many
 // as kChunkBytes hold, so that they stay in L2 while every pair of query tiles
 // reads them; rather fewer than chunks of different sizes, whose last one would
-// leave SMs without work.
+// leave SMs without work.  All heads at a time / 20 / 32 / 48 / 64 / 96 MB: 16
+// prompts of 1,000 to 4,096 tokens (32 + 8 heads, 168 MB) 748 / 709 / 709 / 695 /
+// 697 / 708 us, two of 8,192 (32 + 32 heads, 268 MB) 956 / 959 / 935 / 960 / 914
+// / 925 us.
 int head_chunk(int64_t tokens, int kv_heads) {
   const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kv_heads, kChunkBytes / (tokens * 512)));
   for (int n = most; 2 * n > most; --n)
