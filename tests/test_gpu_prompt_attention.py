@@ -90,6 +90,19 @@ def test_long_prompts(lens, h, group) -> None:
     _check(out, _reference(q, k, v, lens), tokens)
 
 
+@pytest.mark.parametrize("h,group", [(7, 1), (9, 2), (5, 4)])
+def test_more_keys_than_are_walked_at_a_time(h, group) -> None:
+    """Heads in chunks of four and three, three, and four and one."""
+    lens = [50] * 400 + [0, 1, 300] * 30 + [700]
+    tokens = sum(lens)
+    assert 4 <= (64 << 20) // (tokens * 512) < 5
+    q, k, v = _inputs(tokens, h, group, seed=17)
+    out = torch.full((tokens, h * group, DIM), float("nan"), dtype=torch.bfloat16, device="cuda")
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    _check(out, _reference(q, k, v, lens), tokens)
+    assert prompt_status() == 0
+
+
 @pytest.mark.parametrize("layout", ["heads outermost", "padded rows"])
 @pytest.mark.parametrize("h,group", [(2, 4), (1, 2)])
 def test_strided_tensors(layout, h, group) -> None:
