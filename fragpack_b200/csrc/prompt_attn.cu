@@ -27,10 +27,10 @@
 // 80 / 4 each, the 32 whatever the width), an O product five of 64; that is 736
 // cycles where the arithmetic alone is 640, so the products reach at most
 // 0.87 of the tensor cores' rate.  Measured: 1,340 to 1,360 TFLOP/s in short runs
-// on that prompt (0.82 to 0.83 of 1,643), 1,176 without a pause, where the card's
+// on that prompt (0.82 to 0.83 of 1,643), 1,170 without a pause, where the card's
 // power limit holds the clock near 1.4 GHz (0.84 of the 1,400 that plain products
-// keep up); 1,050 to 1,090 on 16 prompts of 1,000 to 4,096 tokens (32 + 8 heads,
-// 730 to 760 us); 46 us for 64 prompts of up to 300 tokens, where an item is too
+// keep up); 1,120 to 1,140 on 16 prompts of 1,000 to 4,096 tokens (32 + 8 heads,
+// 695 to 710 us); 48 us for 64 prompts of up to 300 tokens, where an item is too
 // short to hide its own start.  8,192 tokens (32 + 8 heads) under counters: tensor
 // pipe active 67 %, issue slots 44 %, special-function unit about half, 103 MB
 // read from DRAM and 34 MB written (the results stay in L2 for the next reader).
