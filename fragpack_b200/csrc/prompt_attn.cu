@@ -684,10 +684,12 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
   uint32_t s_used = 0, sums = 0;
   // Tile 0's warp and tile 1's of the same rows sit on one scheduler and take
   // turns at the exponentials, tile 0 first: side by side both would be slow,
-  // and the tensor cores would wait for both.
+  // and the tensor cores would wait for both.  The turn is passed on at half of
+  // them, so that the other's are there when these end (one prompt of 32,768
+  // tokens, 8 + 1 heads: 1,592 us, at the end 1,608, at a third 1,605).
   uint32_t turns = 0;
   const auto take_turn = [&] {
-    if (mine == 1 || turns > 0) await(&sm.turn[mine][rows], (mine == 1 ? turns : turns - 1) & 1u, &sm.wait);
+    await(&sm.turn[mine][rows], (turns + (uint32_t)mine + 1) & 1u, &sm.wait);  // tile 0's first passes at once
     ++turns;
   };
   Item w;
@@ -748,6 +750,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
       uint32_t packed[kKeys / 2];
 #pragma unroll
       for (int i = 0; i < kKeys / 2; ++i) {  // pairs of columns
+        if (i == kKeys / 4 && lane == 0) mbar_arrive(&sm.turn[mine ^ 1][rows]);
         float a, b;
         unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, minus_ref), a, b);
         a = ex2(a);
@@ -755,7 +758,6 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
         row_sum[i & 1] = add2(row_sum[i & 1], pack2(a, b));
         packed[i] = bf16_pair(a, b);
       }
-      arrive_warp(&sm.turn[mine ^ 1][rows], lane);
       if (s_used > 1) await(&sm.p_free[mine], s_used & 1u, &sm.wait);
       tmem_acquire();
       tmem_store<kKeys / 2>(tmem_p, packed);
