@@ -26,14 +26,14 @@
 // What bounds it: an S product of 128 rows takes eight steps of 52 cycles (32 +
 // 80 / 4 each, the 32 whatever the width), an O product five of 64; that is 736
 // cycles where the arithmetic alone is 640, so the products reach at most
-// 0.87 of the tensor cores' rate.  Measured: 1,340 to 1,360 TFLOP/s in short runs
-// on that prompt (0.82 to 0.83 of 1,643), 1,170 without a pause, where the card's
-// power limit holds the clock near 1.4 GHz (0.84 of the 1,400 that plain products
-// keep up); 1,120 to 1,140 on 16 prompts of 1,000 to 4,096 tokens (32 + 8 heads,
-// 695 to 710 us); 48 us for 64 prompts of up to 300 tokens, where an item is too
+// 0.87 of the tensor cores' rate.  Measured: 1,381 TFLOP/s in short runs on that
+// prompt (1,592 us, 0.84 of 1,643), 1,170 to 1,210 without a pause, where the
+// card's power limit holds the clock near 1.4 GHz (0.84 to 0.87 of the 1,400 that
+// plain products keep up); 1,158 on 16 prompts of 1,000 to 4,096 tokens (32 + 8
+// heads, 689 us); 48 us for 64 prompts of up to 300 tokens, where an item is too
 // short to hide its own start.  8,192 tokens (32 + 8 heads) under counters: tensor
-// pipe active 67 %, issue slots 44 %, special-function unit about half, 103 MB
-// read from DRAM and 34 MB written (the results stay in L2 for the next reader).
+// pipe active 68 %, issue slots 44 %, special-function unit about half, 103 MB
+// read from DRAM and 32 MB written (the results stay in L2 for the next reader).
 //
 // One CTA per SM at a time, which goes from item to item; its warps meet only
 // through mbarriers, and every wait is bounded and reports through the status
@@ -90,7 +90,7 @@ constexpr int kSoftmaxRegs = 184, kResultRegs = 88, kOtherRegs = 56;
 // a result relative to attention in FP32 with one rounding, and times on one
 // prompt of 32,768 tokens / on 16 ragged ones: 8: 1.34, 1,638 / 756 us; 4: 1.22,
 // 1,709 / 831; 2: 1.16, 1,749 / 869; 1: 1.13, 1,780 / 882 (a rescale waits for
-// the O product before it).
+// the O product before it; before the last steps, which took 3 to 9 % off all).
 constexpr float kRescaleSlack = 8.f;
 
 __device__ int32_t g_prompt_status;
