@@ -690,6 +690,11 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
   uint32_t turns = 0;
   const auto take_turn = [&] {
     await(&sm.turn[mine][rows], (turns + (uint32_t)mine + 1) & 1u, &sm.wait);  // tile 0's first passes at once
+    // Lane 0 passes the turn on alone.  Without this, a lane still polling could find
+    // that the turn had come back, its barrier's parity where it was, and poll on.
+    // (The other waits are followed by a meeting of the warp before it arrives
+    // anywhere.)
+    __syncwarp();
     ++turns;
   };
   Item w;
