@@ -149,6 +149,7 @@ struct PromptParams {
   float scale_log2;
   uint32_t wait_limit;
   int skip_tile;  // test hook: this K tile of an item is not loaded (-1: none)
+  int falling_blocks;  // test hook: blocks are numbered from the last one down
 };
 
 __device__ __forceinline__ uint32_t clock32() {
@@ -286,8 +287,8 @@ __device__ __forceinline__ void commit(uint64_t* bar, bool wanted = true) {
 // Finds items by their number, one warp.  They are numbered head_chunk KV heads
 // after head_chunk KV heads and within those in the order "all prompts' pairs i,
 // from the largest i down", so that the longest are under way first; the warp
-// walks down the levels i, and within one through the prompts, so numbers must
-// not fall from call to call.
+// walks down the levels i, and within one through the prompts, and begins again
+// should a number fall from call to call (see ask_for_block).
 struct ItemPicker {
   const PromptParams& p;
   PromptSmem& sm;
@@ -298,6 +299,7 @@ struct ItemPicker {
   uint32_t above = 0, here = 0;    // pairs of the levels done; prompts that have one of this level
   int group = 0;                   // prompts 32 group .. are next,
   uint32_t before = 0;             // and so many before them have a pair of this level
+  uint32_t latest = 0;             // number of the last call
 
   __device__ __forceinline__ int2 read_prompt(int r) const {  // first row and rows
     int2 x = make_int2(0, 0);
@@ -335,6 +337,12 @@ struct ItemPicker {
   }
   // Item number `at`; head -1: there are fewer.
   __device__ __forceinline__ Item item(uint32_t at) {
+    if (at < latest) {
+      level = levels;
+      head0 = 0;
+      first = above = here = 0;
+    }
+    latest = at;
     while (head0 < p.kv_heads && at - first >= in_chunk) {
       first += in_chunk;
       head0 += p.head_chunk;
@@ -384,7 +392,9 @@ struct ItemPicker {
 // load warp has begun with the last one taken and the result warps with the one
 // before: asked for earlier, it would be bound to a CTA that may be late (two
 // prompts of 8,192 tokens, 32 + 32 heads: 930 us without the wait for the load
-// warp, 899 with it; without a pause 1,051 / 1,029).
+// warp, 899 with it; without a pause 1,051 / 1,029).  Blocks come in rising order
+// as a rule, but nothing promises it: whatever order they come in, every one is
+// looked at, also behind one that has no item.
 __device__ __forceinline__ void ask_for_block(PromptSmem& sm, int lane) {
   if (lane == 0) {
     mbar_expect_tx(&sm.block_full, 16);
@@ -415,29 +425,34 @@ __device__ __forceinline__ void prompt_items(const PromptParams& p, PromptSmem& 
   ItemPicker picker(p, sm, lane);
   uint32_t number = blockIdx.x, asked = 0;
   bool more = true, answered = true;  // `number` is a block of this CTA's
-  for (int n = 0;; ++n) {
-    const int slot = n & 1;
-    if (n >= 2 && !await_all(&sm.item_empty[slot], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) break;
-    if (n > 0) {
-      if (!await_all(&sm.item_wanted, (uint32_t)(n - 1) & 1u, &sm.wait)) break;
-      ask_for_block(sm, lane);
-      answered = await_all(&sm.block_full, asked++ & 1u, &sm.wait);
-      if (!answered) break;
-      more = block_taken(sm, number);
-    }
-    Item w;
-    w.head = -1;
-    if (more) w = picker.item(number);
+  int n = 0;                          // items so far
+  const auto publish = [&](const Item& w) {
     if (lane == 0) {
-      sm.item[slot] = w;
-      mbar_arrive(&sm.item_full[slot]);
+      sm.item[n & 1] = w;
+      mbar_arrive(&sm.item_full[n & 1]);
     }
     __syncwarp();
-    if (w.head < 0) break;
+    ++n;
+  };
+  while (more) {
+    const Item w = picker.item(p.falling_blocks ? gridDim.x - 1 - number : number);
+    if (w.head >= 0) {
+      publish(w);
+      if (n >= 2 && !await_all(&sm.item_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, &sm.wait)) break;
+      if (!await_all(&sm.item_wanted, (uint32_t)(n - 1) & 1u, &sm.wait)) break;
+    }
+    ask_for_block(sm, lane);
+    answered = await_all(&sm.block_full, asked++ & 1u, &sm.wait);
+    if (!answered) break;
+    more = block_taken(sm, number);
   }
-  // Blocks that are left have no item (or a wait ran out, and the call is
-  // invalid): they are taken all the same, beside the last items, so that none of
-  // them has to start.
+  if (!more) {
+    Item none;
+    none.head = -1;
+    publish(none);
+  }
+  // A wait ran out, and the call is invalid: the blocks that are left are taken all
+  // the same, so that none of them has to start.
   while (more) {
     if (answered) {
       ask_for_block(sm, lane);
@@ -1072,6 +1087,11 @@ int head_chunk(int64_t tokens, int kv_heads) {
   return most;
 }
 
+std::atomic<int>& falling_blocks() {
+  static std::atomic<int> on{0};
+  return on;
+}
+
 bool strides_fit(const void* base, int64_t tokens, int64_t heads, int64_t token_stride, int64_t head_stride) {
   const auto fits = [](int64_t n, int64_t stride) {
     return n == 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38));
@@ -1125,12 +1145,18 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_limit = (uint32_t)std::min<long long>(wait_debug().limit, 0xf0000000LL);
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
+  p.falling_blocks = falling_blocks().load(std::memory_order_relaxed);
   // Every prompt has at most one pair of tiles that is not full.
   const int64_t items = (tokens / (kQTiles * tile_tokens) + prompts) * kv_heads;
   FP_REQUIRE(items < (1LL << 31), "too much work for one call (%lld tokens, %d prompts, %d KV heads)", (long long)tokens,
              prompts, kv_heads);
   prompt_attn_kernel<<<(unsigned)items, kPromptThreads, smem, (cudaStream_t)stream>>>(p);
   FP_LAUNCH_CHECK("prompt_attn_kernel");
+  return FP_OK;
+}
+
+int fp_debug_falling_blocks(int32_t on) {
+  falling_blocks().store(on != 0, std::memory_order_relaxed);
   return FP_OK;
 }
 

@@ -124,6 +124,7 @@ _SIGNATURES = {
     "fp_hbm_gather": [c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i32, c_ptr],
     "fp_hbm_gather_status": [c_ptr],
     "fp_debug_wait_limit": [c_i64, c_i64],
+    "fp_debug_falling_blocks": [c_i32],
     "fp_hbm_export": [c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i32, c_i32,
                       c_i32, c_i64, c_ptr],
     "fp_hbm_import": [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64,

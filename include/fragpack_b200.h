@@ -381,6 +381,12 @@ int fp_hbm_gather_status(int32_t* status);
  */
 int fp_debug_wait_limit(int64_t cycles, int64_t skip_record);
 
+/* Test hook: fp_prompt_attention's launches that follow number the blocks of
+ * their grid from the last one down (`on` != 0), so that the CTAs that take
+ * blocks over meet their items in falling order.  Results do not depend on it.
+ * Process-wide. */
+int fp_debug_falling_blocks(int32_t on);
+
 /*
  * hbm_export (fragpack/ops/hbm_kv.cu:755-774): closed blocks -> block blobs.
  * Blob i is written at out + i * stride and lengths[i] receives its size (a
