@@ -56,6 +56,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "fp_api.h"
 #include "fp_common.cuh"
@@ -114,6 +115,8 @@ struct PromptSmem {
   __align__(1024) uint8_t k[kStages][kKeyTileBytes];
   __align__(1024) uint8_t v[kStages][kKeyTileBytes];
   float sum[kQTiles][kTile];  // of the probabilities of each row
+  int stray[3][kTile];        // see screen_values
+  int stray_item;             // the item that they belong to
   Item item[2];
   int2 prompts[kKeptPrompts];  // first row and rows of the first prompts
   __align__(16) uint8_t block[16];  // answer to the request for a block
@@ -131,15 +134,8 @@ struct PromptSmem {
   PromptWait wait;
 };
 
-// BF16 [tokens, heads, 128], strides in scalars.
-struct Heads {
-  const __nv_bfloat16* at;
-  int64_t token, head;
-};
-
 struct PromptParams {
   CUtensorMap q_map, k_map, v_map;
-  Heads q, k, v;
   __nv_bfloat16* out;
   int64_t o_token, o_head;
   const int32_t* starts;
@@ -522,13 +518,67 @@ __device__ __forceinline__ void prompt_load(const PromptParams& p, PromptSmem& s
   }
 }
 
-// Rows (tokens) valid .. of a V tile become zero: they belong to another prompt
-// or to nothing, and whatever they hold must not meet a zero probability.
-__device__ __forceinline__ void clear_value_rows(uint8_t* tile, int valid, int lane) {
-  for (int x = valid * 16 + lane; x < kKeys * 16; x += 32) {
-    const int row = x >> 4, chunk = x & 15;
-    *reinterpret_cast<uint4*>(tile + (chunk >> 3) * kKeyHalf + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+// Rows (tokens) from .. of a V tile become zero: no row of the item sees them (they
+// come later, belong to another prompt or to nothing), and whatever they hold must
+// not meet a zero probability.
+__device__ __forceinline__ void clear_value_rows(uint8_t* tile, int from, int lane) {
+#pragma unroll 1
+  for (int x = from * 8 + lane; x < kKeys * 8; x += 32) {
+    reinterpret_cast<uint4*>(tile)[x] = make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(tile + kKeyHalf)[x] = make_uint4(0u, 0u, 0u, 0u);
   }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// The same goes for tokens that only some of an item's rows see: their zero
+// probabilities must not meet an infinity or a NaN.  Do rows from .. to - 1 of a V
+// tile hold one?
+__device__ __forceinline__ bool has_stray_values(const uint8_t* tile, int from, int to, int lane) {
+  uint32_t sum[4] = {0, 0, 0, 0};  // 0 * x of everything, as pairs
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const uint4* const rows = reinterpret_cast<const uint4*>(tile + half * kKeyHalf) + 8 * from;
+    const int count = 8 * (to - from);
+#pragma unroll 1
+    for (int i = lane; i < count; i += 4 * 32) {
+      uint4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = i + 32 * u < count ? rows[i + 32 * u] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(x[u].x), "r"(0u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(x[u].y), "r"(0u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(x[u].z), "r"(0u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(x[u].w), "r"(0u));
+      }
+    }
+  }
+  return __any_sync(0xffffffffu, (sum[0] | sum[1] | sum[2] | sum[3]) != 0);
+}
+
+// Takes all of the tile's out of it (they become zero) and notes in sm.stray, per dim, the
+// first token of the prompt that holds an infinity of either sign and the first
+// that holds a NaN; the result warps bring them back into the rows that see these
+// tokens.  So such values take no time beside the search, which costs 64 short
+// prompts 2 us (48 to 50) and 16 ragged ones 7 (693 to 700); rows that came out NaN
+// computed again one by one took 600 times as long where a prompt of 4,096 tokens
+// held an infinity in its first token.  `fresh`: the first time in this item.
+__device__ __forceinline__ void screen_values(PromptSmem& sm, uint8_t* tile, int token0, bool fresh, int lane) {
+  if (fresh)
+    for (int x = lane; x < 3 * kTile; x += 32) sm.stray[x / kTile][x % kTile] = INT_MAX;
+  __syncwarp();
+#pragma unroll 1
+  for (int x = lane; x < kKeyTileBytes / 2; x += 32) {
+    uint16_t* const at = reinterpret_cast<uint16_t*>(tile) + x;
+    const uint32_t bits = *at;
+    if ((bits & 0x7f80u) != 0x7f80u) continue;
+    const int row = x % (kKeyHalf / 2) / 64, chunk = (x % 64 >> 3) ^ (row & 7);
+    const int dim = x / (kKeyHalf / 2) * 64 + chunk * 8 + (x & 7);
+    atomicMin(&sm.stray[(bits & 0x7fu) ? 2 : bits >> 15][dim], token0 + row);
+    *at = 0;
+  }
+  __threadfence_block();
+  __syncwarp();
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
@@ -575,18 +625,30 @@ __device__ __forceinline__ void issue_scores(PromptSmem& sm, uint32_t tmem, int 
 }
 
 // The warp that issues the value products: O_t(j) as soon as P_t(j) is written.
-__device__ __forceinline__ void issue_values(PromptSmem& sm, uint32_t tmem, int lane) {
+__device__ __forceinline__ void issue_values(PromptSmem& sm, uint32_t tmem, int lane, int group_log2) {
   uint32_t items[kQTiles] = {0, 0}, issued[kQTiles] = {0, 0};
   uint32_t tile = 0;  // key tiles so far
   Item w;
   for (int n = 0; next_item(sm, n, lane, w); ++n) {
     const int last_any = max(w.last[0], w.last[1]);
+    // Tokens up to tok0 are seen by every row of the item, those from `end` on by none.
+    const int end = min(w.tok0 + (kQTiles * kTile >> group_log2), w.length);
+    bool screened = false;
 #pragma unroll 1
     for (int j = 0; j <= last_any; ++j, ++tile) {
       const uint32_t stage = tile % kStages;
       await(&sm.v_full[stage], (tile / kStages) & 1u, &sm.wait);
-      const int valid = w.length - j * kKeys;
-      if (valid < kKeys) clear_value_rows(sm.v[stage], valid, lane);
+      const int to = min(end - j * kKeys, kKeys), from = max(w.tok0 + 1 - j * kKeys, 0);
+      if (to < kKeys) clear_value_rows(sm.v[stage], to, lane);
+      if (from < to && has_stray_values(sm.v[stage], from, to, lane)) {
+        // What is noted of an earlier item has been read once its O has been: of the
+        // tiles that this item has, that is so from its second key tile on.
+        for (int t = 0; t < kQTiles; ++t)
+          if ((j == 0 || w.last[t] < 0) && items[t] > 0) await(&sm.o_free[t], (items[t] - 1) & 1u, &sm.wait);
+        screen_values(sm, sm.v[stage], j * kKeys, !screened, lane);
+        screened = true;
+        if (lane == 0) *reinterpret_cast<volatile int*>(&sm.stray_item) = n;
+      }
 #pragma unroll
       for (int t = 0; t < kQTiles; ++t) {
         if (j > w.last[t]) continue;
@@ -598,7 +660,10 @@ __device__ __forceinline__ void issue_values(PromptSmem& sm, uint32_t tmem, int 
         value_product(tmem + (uint32_t)(t * kTile), tmem + kTmemP + (uint32_t)(t * kKeys / 2),
                       value_desc_low(smem_addr(sm.v[stage])), j > 0);
         commit(&sm.p_free[t]);
-        if (j == w.last[t]) commit(&sm.o_done[t]);
+        if (j == w.last[t]) {
+          commit(&sm.o_done[t]);
+          arrive_warp(&sm.o_done[t], lane);  // for what screen_values wrote
+        }
       }
       commit(&sm.v_empty[stage]);
     }
@@ -726,6 +791,9 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
     const int position = min(w.tok0 + ((mine * kTile + row) >> p.group_log2), w.length - 1);
     // Key tiles below this one are seen whole by every row.
     const int first_masked = (w.tok0 + (mine * kTile >> p.group_log2) + 1) / kKeys;
+    // Weights are 2^-shift smaller, so that they sum to less than a half (each is
+    // below 2^kRescaleSlack otherwise) and no sum of finite values overflows.
+    const float shift = kRescaleSlack + 1.f + (float)(32 - __clz(w.length));
     float ref = 0.f;  // reference point of the exponentials
     uint64_t row_sum[2] = {0, 0};
 #pragma unroll 1
@@ -772,7 +840,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
           }
         }
       }
-      const uint64_t minus_ref = pack2(-ref, -ref);
+      const uint64_t minus_ref = pack2(-ref - shift, -ref - shift);
       take_turn();
       uint32_t packed[kKeys / 2];
 #pragma unroll
@@ -809,75 +877,6 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
 // ---------------------------------------------------------------------------
 // Results.
 
-// One query row by one warp over the keys that it sees, kRowKeys at a time, lane
-// l carrying dims 4 l .. 4 l + 3.  The tensor cores also multiply the values of
-// later tokens (by zero probabilities), so a row that came out NaN or infinite
-// from a sound sum is computed again here: what it then shows is its own.  Its
-// weights are 2^-kRowShift smaller, so that no sum of finite values overflows.
-constexpr int kRowKeys = 2;
-constexpr float kRowShift = 32.f;  // tokens are fewer than 2^30
-
-__device__ __forceinline__ void prompt_row(const PromptParams& p, int row0, int tok, int kv_head, int q_head, int lane) {
-  const auto load = [&](const Heads& h, int row, int head) {
-    return *reinterpret_cast<const uint2*>(h.at + row * h.token + head * h.head + 4 * lane);
-  };
-  const auto widen = [](uint2 two, float (&x)[4]) {
-    x[0] = __uint_as_float(two.x << 16);
-    x[1] = __uint_as_float(two.x & 0xffff0000u);
-    x[2] = __uint_as_float(two.y << 16);
-    x[3] = __uint_as_float(two.y & 0xffff0000u);
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-  widen(load(p.q, row0 + tok, q_head), q);
-#pragma unroll 1
-  for (int j0 = 0; j0 <= tok; j0 += kRowKeys) {
-    uint2 keys[kRowKeys], values[kRowKeys];
-    float score[kRowKeys], new_top = top;
-#pragma unroll
-    for (int u = 0; u < kRowKeys; ++u) {
-      const int row = row0 + min(j0 + u, tok);
-      keys[u] = load(p.k, row, kv_head);
-      values[u] = load(p.v, row, kv_head);
-    }
-#pragma unroll
-    for (int u = 0; u < kRowKeys; ++u) {
-      float k[4];
-      widen(keys[u], k);
-      score[u] = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1)
-#pragma unroll
-      for (int u = 0; u < kRowKeys; ++u) score[u] += __shfl_xor_sync(0xffffffffu, score[u], d);
-#pragma unroll
-    for (int u = 0; u < kRowKeys; ++u) {
-      score[u] = j0 + u <= tok ? score[u] * p.scale_log2 : -INFINITY;
-      new_top = fmaxf(new_top, score[u]);
-    }
-    const float ref = new_top == -INFINITY ? 0.f : new_top;
-    if (new_top > top) {
-      const float keep = ex2(top - ref);
-      sum *= keep;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) o[x] *= keep;
-      top = new_top;
-    }
-#pragma unroll
-    for (int u = 0; u < kRowKeys; ++u) {
-      const float weight = ex2(score[u] - ref - kRowShift);
-      float v[4];
-      widen(values[u], v);
-      sum += weight;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (weight != 0.f) o[x] += weight * v[x];  // also for NaN
-    }
-  }
-  const float inv = sum > 0.f ? 1.f / sum : sum;
-  *reinterpret_cast<uint2*>(p.out + (row0 + tok) * p.o_token + q_head * p.o_head + 4 * lane) =
-      make_uint2(bf16_pair(o[0] * inv, o[1] * inv), bf16_pair(o[2] * inv, o[3] * inv));
-}
-
 // Result warps: thread = query row of both tiles.
 __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem& sm, uint32_t tmem, int row) {
   const int lane = row & 31;
@@ -898,7 +897,6 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
       // Rows go out through shared memory, so that they leave in whole lines; a
       // warp keeps to its 32 rows.
       const uint64_t inv2 = pack2(inv, inv);
-      uint64_t stray = 0;  // becomes NaN with any infinite or NaN result
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 32) {
         uint32_t o[32];
@@ -909,12 +907,27 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const uint64_t y = fma2(pack2(__uint_as_float(o[8 * ch + 2 * x]), __uint_as_float(o[8 * ch + 2 * x + 1])), inv2, 0);
-            stray = fma2(y, 0, stray);
             float a, b;
             unpack2(y, a, b);
             packed[x] = bf16_pair(a, b);
           }
           *reinterpret_cast<uint4*>(sm.o + tile_chunk(row, c + 8 * ch)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        }
+      }
+      if (*reinterpret_cast<volatile int*>(&sm.stray_item) == n) {
+        // The infinities and NaN that were taken out of the values, for the rows
+        // that see them: there every weight is positive.
+        __threadfence_block();
+        const int token = w.tok0 + ((t * kTile + row) >> p.group_log2);
+#pragma unroll 1
+        for (int d = 0; d < kTile; ++d) {
+          const bool up = sm.stray[0][d] <= token, down = sm.stray[1][d] <= token;
+          float add = up ? INFINITY : down ? -INFINITY : 0.f;
+          if (sm.stray[2][d] <= token || (up && down)) add = NAN;
+          if (add == 0.f) continue;
+          uint16_t* const at = reinterpret_cast<uint16_t*>(sm.o + tile_chunk(row, d)) + (d & 7);
+          const float y = __uint_as_float((uint32_t)*at << 16) + add;
+          *at = (uint16_t)bf16_pair(y, y);
         }
       }
       tmem_release();
@@ -940,16 +953,7 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
         tok += on ? tokens : 0;
         g = on ? g & (p.group - 1) : g;
       }
-      float a, b;
-      unpack2(stray, a, b);
-      // A NaN among the scores that a row sees makes its sum NaN, and the row with it.
-      const bool finite =
-          (a == 0.f && b == 0.f) || sum != sum || w.tok0 + ((t * kTile + row) >> p.group_log2) >= w.length;
       __syncwarp();
-      for (uint32_t again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
-        const int r = first_row + __ffs(again) - 1;
-        prompt_row(p, w.row0, w.tok0 + (r >> p.group_log2), w.head, w.head * p.group + (r & (p.group - 1)), lane);
-      }
     }
   }
 }
@@ -984,13 +988,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
       for (int i = 0; i < 4; ++i) mbar_init(&sm.turn[t][i], 1);
       mbar_init(&sm.sum_full[t], 4);
       mbar_init(&sm.sum_empty[t], kResultWarps);
-      mbar_init(&sm.o_done[t], 1);
+      mbar_init(&sm.o_done[t], 2);  // the products and the value warp
       mbar_init(&sm.o_free[t], kResultWarps);
     }
     mbar_init(&sm.item_wanted, 1);
     mbar_init(&sm.block_full, 1);
     mbar_init(&sm.drained[0], 1);
     mbar_init(&sm.drained[1], 1);
+    sm.stray_item = -1;
     sm.wait.abort = 0;
     sm.wait.limit = p.wait_limit;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1019,7 +1024,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kScoreWarp) issue_scores(sm, tmem, lane);
-    if (warp == kValueWarp) issue_values(sm, tmem, lane);
+    if (warp == kValueWarp) issue_values(sm, tmem, lane, p.group_log2);
     if (warp == kLoadWarp) prompt_load(p, sm, lane);
     if (warp == kItemWarp) prompt_items(p, sm, lane);
   }
@@ -1129,9 +1134,6 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   static std::atomic<uint64_t> smem_allowed;
   const int smem = (int)sizeof(PromptSmem) + 1024;
   if (int rc = allow_dynamic_smem(prompt_attn_kernel, smem, smem_allowed)) return rc;
-  p.q = Heads{static_cast<const __nv_bfloat16*>(q), q_token, q_head};
-  p.k = Heads{static_cast<const __nv_bfloat16*>(k), k_token, k_head};
-  p.v = Heads{static_cast<const __nv_bfloat16*>(v), v_token, v_head};
   p.out = static_cast<__nv_bfloat16*>(out);
   p.o_token = o_token;
   p.o_head = o_head;

@@ -34,7 +34,8 @@ def prompt_attention(
     Prompt ``r`` owns the rows ``starts[r] .. starts[r + 1]`` of all four
     tensors; each of its rows sees the prompt's rows up to and including
     itself.  Rows outside every prompt are left as they were, and what they
-    hold reaches no result.
+    hold reaches no result.  Infinities and NaN reach the rows that see them and
+    no others, and take no more time than other values.
 
     Args:
         q: BF16 ``[T, H * G, 128]`` queries.

@@ -33,3 +33,100 @@ def test_blocks_in_falling_order(lens, h, group) -> None:
     _check(rising, _reference(q, k, v, lens), tokens)
     assert torch.equal(rising, falling)
     assert prompt_status() == 0
+
+
+def _stray_reference(q, k, v, lens):
+    """As ``_reference``, infinities and NaN of the values added where a row sees them (every weight is positive)."""
+    out, tolerance = _reference(q, k, torch.where(torch.isfinite(v), v, torch.zeros_like(v)), lens)
+    group, t0 = q.shape[1] // k.shape[1], 0
+    for n in lens:
+        rows = slice(t0, t0 + n)
+        up, down, nan = (torch.cummax(x[rows].int(), 0).values.bool().repeat_interleave(group, 1) if n else x[rows]
+                         for x in (v == float("inf"), v == float("-inf"), torch.isnan(v)))
+        if n:
+            part = out[rows]
+            part[up & ~down] = float("inf")
+            part[down & ~up] = float("-inf")
+            part[nan | (up & down)] = float("nan")
+        t0 += n
+    return out, tolerance
+
+
+def _check_stray(got, want) -> None:
+    out, tolerance = want
+    got = got.double()
+    for kind in (torch.isnan, lambda x: x == float("inf"), lambda x: x == float("-inf")):
+        assert torch.equal(kind(got), kind(out))
+    sound = torch.isfinite(out)
+    assert bool(((got - out).abs() <= tolerance)[sound].all())
+
+
+@pytest.mark.parametrize("h,group", [(2, 1), (3, 2), (2, 8)])
+@pytest.mark.parametrize("lens,every", [
+    ([400], 40), ([700, 3, 1025], 97), ([1, 80, 79, 160, 81] * 30, 50), ([300] * 160 + [0, 7] * 20, 333), ([257], 1),
+    ([513, 600], 3000),
+])
+def test_stray_values_show_in_the_rows_that_see_them_alone(lens, every, h, group) -> None:
+    """Infinities of both signs and NaN in single dims of about one token in `every`, many items of a CTA among them."""
+    tokens = sum(lens)
+    q, k, v = _inputs(tokens, h, group, seed=every)
+    gen = torch.Generator().manual_seed(every)
+    for head in range(h):
+        for t in torch.randperm(tokens, generator=gen)[: max(3, tokens // every)].tolist():
+            dim = int(torch.randint(0, DIM, (1,), generator=gen))
+            v[t, head, dim] = (float("inf"), float("-inf"), float("nan"))[t % 3]
+    out = torch.zeros(tokens, h * group, DIM, dtype=torch.bfloat16, device="cuda")
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    _check_stray(out, _stray_reference(q, k, v, lens))
+    assert prompt_status() == 0
+
+
+@pytest.mark.parametrize("what", ["first inf", "last nan", "all inf", "all nan", "large"])
+def test_stray_values_take_the_time_of_sound_ones(what) -> None:
+    n, h, group = 4096, 2, 8
+    q, k, v = _inputs(n, h, group, seed=21)
+    bad = v.clone()
+    if what == "large":
+        bad = bad.sign() * 3e38
+    else:
+        where, value = what.split()
+        bad[{"first": 0, "last": n - 1, "all": slice(None)}[where]] = float(value)
+    out, starts = torch.zeros_like(q), _starts([n])
+
+    def milliseconds(values):
+        best = float("inf")
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            prompt_attention(q, k, values, starts, SCALE, out)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        return best
+
+    sound = milliseconds(v)
+    assert milliseconds(bad) <= 2.0 * sound + 0.02
+    _check_stray(out, _stray_reference(q, k, bad, [n]))
+
+
+def test_values_of_the_largest_size() -> None:
+    """Their weighted mean is in range, whatever their sums are, in prompts of any length."""
+    lens = [1, 90, 2000, 5]
+    q, k, v = _inputs(sum(lens), 2, 4, seed=22)
+    v = v.sign() * 3e38
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    _check(out, _reference(q, k, v, lens), sum(lens))
+
+
+def test_one_infinity_in_a_very_long_prompt() -> None:
+    n = 140_000
+    q, k, v = _inputs(n, 1, 8, seed=23)
+    want = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts([n]), SCALE, want)
+    v[0, 0, 3], v[n - 50, 0, 4] = float("inf"), float("-inf")
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts([n]), SCALE, out)
+    assert prompt_status() == 0
+    want[..., 3], want[n - 50 :, :, 4] = float("inf"), float("-inf")
+    assert torch.equal(out, want)
