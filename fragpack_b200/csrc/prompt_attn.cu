@@ -56,6 +56,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "fp_api.h"
@@ -818,7 +819,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
         // An infinite or NaN maximum makes the whole row NaN.
         if (!(tile_max < INFINITY)) tile_max = NAN;
         if (j == 0) {
-          ref = tile_max == -INFINITY ? 0.f : tile_max;
+          ref = tile_max == -INFINITY ? -FLT_MAX : tile_max;  // below every score to come
         } else {
           float keep = 1.f;
           if (!(tile_max <= ref + kRescaleSlack)) {
@@ -893,7 +894,7 @@ __device__ __forceinline__ void prompt_results(const PromptParams& p, PromptSmem
       await(&sm.o_done[t], (used >> t) & 1u, &sm.wait);
       used ^= 1u << t;
       tmem_acquire();
-      const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays NaN
+      const float inv = 1.f / sum;  // sum 0: every score is -inf, and the row NaN
       // Rows go out through shared memory, so that they leave in whole lines; a
       // warp keeps to its 32 rows.
       const uint64_t inv2 = pack2(inv, inv);

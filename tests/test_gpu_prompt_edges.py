@@ -130,3 +130,20 @@ def test_one_infinity_in_a_very_long_prompt() -> None:
     assert prompt_status() == 0
     want[..., 3], want[n - 50 :, :, 4] = float("inf"), float("-inf")
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("group", [1, 8])
+@pytest.mark.parametrize("low", [-4.0, -500.0])
+def test_scores_of_minus_infinity(group, low) -> None:
+    """Rows that see only such scores are NaN, as the definition has it; later ones ignore them, however low theirs are."""
+    n, first = 300, 101
+    q, k, v = _inputs(n, 1, group, seed=24)
+    q[:], k[:] = 0.0, 0.0
+    q[..., 0] = 8.0
+    k[:first, 0, 0] = float("-inf")
+    k[first:, 0, 0] = low + torch.arange(n - first, device="cuda") / 64.0
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts([n]), SCALE, out)
+    want, tolerance = _reference(q, k, v, [n])
+    assert bool(torch.isnan(want[:first]).all()) and bool(torch.isnan(out[:first]).all())
+    _check(out[first:], (want[first:], tolerance[first:]), n - first)
