@@ -1165,6 +1165,8 @@ int fp_debug_falling_blocks(int32_t on) {
 
 int fp_prompt_status(int32_t* status) {
   FP_REQUIRE(status, "null status");
+  // The copies below go by the legacy stream, which non-blocking streams do not wait for.
+  if (int rc = cuda_status(cudaDeviceSynchronize(), "cudaDeviceSynchronize")) return rc;
   if (int rc = cuda_status(cudaMemcpyFromSymbol(status, g_prompt_status, sizeof(int32_t)),
                            "cudaMemcpyFromSymbol(g_prompt_status)"))
     return rc;

@@ -278,8 +278,8 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
                         void* out, int64_t o_token, int64_t o_head, int32_t kv_heads, int32_t group,
                         float scale, void* stream);
 
-/* Copies the prompt kernel's status word to the host (synchronises the device's
- * prior work on the legacy stream) and clears it. */
+/* Copies the prompt kernel's status word to the host (synchronises the device, so
+ * that every call made before it has reported) and clears it. */
 int fp_prompt_status(int32_t* status);
 
 /*

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from fragpack_b200.ops.fragpack_ext import check, extension
-from fragpack_b200.ops.prompt_attn import prompt_attention, prompt_status
+from fragpack_b200.ops.prompt_attn import PROMPT_WAIT_TIMEOUT, prompt_attention, prompt_status
 from tests.test_gpu_prompt_attention import DIM, SCALE, _check, _inputs, _reference, _starts
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +147,21 @@ def test_scores_of_minus_infinity(group, low) -> None:
     want, tolerance = _reference(q, k, v, [n])
     assert bool(torch.isnan(want[:first]).all()) and bool(torch.isnan(out[:first]).all())
     _check(out[first:], (want[first:], tolerance[first:]), n - first)
+
+
+def test_status_of_a_call_on_another_stream() -> None:
+    """Reading the status waits for calls on every stream of the device: this one reports after some 40 ms."""
+    q, k, v = _inputs(500, 2, 8, seed=8)
+    starts, out = _starts([500]), torch.zeros_like(q)
+    assert prompt_status() == 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    check(extension().fp_debug_wait_limit(80_000_000, 1))
+    try:
+        with torch.cuda.stream(side):
+            prompt_attention(q, k, v, starts, SCALE, out)
+        assert prompt_status() == PROMPT_WAIT_TIMEOUT
+    finally:
+        check(extension().fp_debug_wait_limit(0, -1))
+    torch.cuda.synchronize()
+    assert prompt_status() == 0
