@@ -71,6 +71,6 @@ def test_a_wait_that_ends_a_loop_ends_it_for_the_whole_warp() -> None:
     """A lane that saw the wait give up must not leave a loop that the others go on with: the warp meets in it."""
     text = SOURCE.read_text()
     load = text.index("void prompt_load(")  # one lane's waits
-    code = text[text.index("void prompt_items(") : load] + text[text.index("// Rows (tokens) valid .. of a V tile") :]
+    code = text[text.index("void prompt_items(") : load] + text[text.index("void issue_scores(") :]
     deciding = [line.strip() for line in code.splitlines() if re.search(r"(!|=\s*|return\s+|&&\s*)await\(", line)]
     assert not deciding
