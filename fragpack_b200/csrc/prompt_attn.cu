@@ -86,14 +86,15 @@ static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "
 // + 128 x 88 + 128 x 56 = 512 x 128, what the block is launched with.
 constexpr int kSoftmaxRegs = 184, kResultRegs = 88, kOtherRegs = 56;
 // How far (log2 units) a row's maximum may rise above the reference point of its
-// exponentials before the reference follows and O is rescaled.  Nothing is lost
-// in range (a weight stays below 2^8, a sum below 2^38), but the largest weights,
-// rounded to BF16, no longer include the exact 1 of a row's maximum.  RMS error of
-// a result relative to attention in FP32 with one rounding, and times on one
-// prompt of 32,768 tokens / on 16 ragged ones: 8: 1.34, 1,638 / 756 us; 4: 1.22,
-// 1,709 / 831; 2: 1.16, 1,749 / 869; 1: 1.13, 1,780 / 882 (a rescale waits for
-// the O product before it; before the last steps, which took 3 to 9 % off all).
-constexpr float kRescaleSlack = 8.f;
+// exponentials before the reference follows and O is rescaled: the caller's choice,
+// up to this.  Nothing is lost in range, but the largest weights, rounded to BF16, no
+// longer include the exact 1 of a row's maximum.  RMS error against 64 bits relative to that
+// of attention in FP32 with one rounding (five sets of prompts of 1 to 16,384 tokens),
+// and times of 16 ragged prompts / of one of 32,768 tokens: 8: 1.16 to 1.34, 710 /
+// 1,616 us; 4: 1.15 to 1.22, 794 / 1,680; 2: 1.13 to 1.17, 829 / 1,714; 1: 1.12 to
+// 1.14, 842 / 1,750; 0: 1.08 to 1.12, 859 / 1,835 (a rescale waits for the O product
+// before it).  Largest error at 8: up to 1.9 times that of FP32, at 0 up to 1.2 times.
+constexpr float kLongestLag = 8.f;
 
 __device__ int32_t g_prompt_status;
 
@@ -143,7 +144,7 @@ struct PromptParams {
   int prompts, tokens, kv_heads;
   int head_chunk;  // KV heads whose items come before the next ones'
   int group, group_log2;
-  float scale_log2;
+  float scale_log2, lag;
   uint32_t wait_limit;
   int skip_tile;  // test hook: this K tile of an item is not loaded (-1: none)
   int falling_blocks;  // test hook: blocks are numbered from the last one down
@@ -793,8 +794,8 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
     // Key tiles below this one are seen whole by every row.
     const int first_masked = (w.tok0 + (mine * kTile >> p.group_log2) + 1) / kKeys;
     // Weights are 2^-shift smaller, so that they sum to less than a half (each is
-    // below 2^kRescaleSlack otherwise) and no sum of finite values overflows.
-    const float shift = kRescaleSlack + 1.f + (float)(32 - __clz(w.length));
+    // below 2^lag otherwise) and no sum of finite values overflows.
+    const float shift = p.lag + 1.f + (float)(32 - __clz(w.length));
     float ref = 0.f;  // reference point of the exponentials
     uint64_t row_sum[2] = {0, 0};
 #pragma unroll 1
@@ -814,15 +815,15 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
         top[(x >> 1) & 3] = max3(top[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
       // The scale is positive, so the largest raw score gives the largest scaled one.
       float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
-      // The reference follows the running maximum once that is kRescaleSlack above it.
-      if (__any_sync(0xffffffffu, j == 0 || !(tile_max <= ref + kRescaleSlack))) {
+      // The reference follows the running maximum once that is p.lag above it.
+      if (__any_sync(0xffffffffu, j == 0 || !(tile_max <= ref + p.lag))) {
         // An infinite or NaN maximum makes the whole row NaN.
         if (!(tile_max < INFINITY)) tile_max = NAN;
         if (j == 0) {
           ref = tile_max == -INFINITY ? -FLT_MAX : tile_max;  // below every score to come
         } else {
           float keep = 1.f;
-          if (!(tile_max <= ref + kRescaleSlack)) {
+          if (!(tile_max <= ref + p.lag)) {
             keep = ex2(ref - tile_max);
             ref = tile_max;
             row_sum[0] = fma2(row_sum[0], pack2(keep, keep), 0);
@@ -1116,11 +1117,20 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
                         const void* v, int64_t v_token, int64_t v_head, const int32_t* starts, int32_t prompts,
                         int64_t tokens, void* out, int64_t o_token, int64_t o_head, int32_t kv_heads, int32_t group,
                         float scale, void* stream) {
+  return fp_prompt_attention_lag(q, q_token, q_head, k, k_token, k_head, v, v_token, v_head, starts, prompts, tokens, out,
+                                 o_token, o_head, kv_heads, group, scale, kLongestLag, stream);
+}
+
+int fp_prompt_attention_lag(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                            int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* starts,
+                            int32_t prompts, int64_t tokens, void* out, int64_t o_token, int64_t o_head,
+                            int32_t kv_heads, int32_t group, float scale, float lag, void* stream) {
   if (prompts == 0 || tokens == 0) return FP_OK;
   FP_REQUIRE(prompts > 0 && tokens > 0 && tokens < (1LL << 30) && kv_heads > 0 && kv_heads <= 65535,
              "bad prompt geometry (%d prompts, %lld tokens, %d KV heads)", prompts, (long long)tokens, kv_heads);
   FP_REQUIRE(group == 1 || group == 2 || group == 4 || group == 8, "query group %d must be 1, 2, 4 or 8", group);
   FP_REQUIRE(scale > 0.f && scale < INFINITY, "the softmax scale must be positive and finite");
+  FP_REQUIRE(lag >= 0.f && lag <= kLongestLag, "the lag must be within 0 .. %g", kLongestLag);
   FP_REQUIRE(q && k && v && starts && out, "null prompt attention argument");
   const int q_heads = kv_heads * group;
   FP_REQUIRE(strides_fit(q, tokens, q_heads, q_token, q_head) && strides_fit(k, tokens, kv_heads, k_token, k_head) &&
@@ -1146,6 +1156,7 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
   p.group = group;
   p.group_log2 = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.lag = lag;
   p.wait_limit = (uint32_t)std::min<long long>(wait_debug().limit, 0xf0000000LL);
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));
   p.falling_blocks = falling_blocks().load(std::memory_order_relaxed);

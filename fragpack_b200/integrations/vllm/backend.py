@@ -331,7 +331,8 @@ def run_layer(
     for group, over_prompt in zip(md.prefills, direct):
         rows = slice(group.tok0, group.tok1)
         if over_prompt:
-            prompt_attention(query[rows], key[rows], value[rows], group.cu_seqlens_q, scale, output[rows])
+            # Weights as precise as those of the path over the records.
+            prompt_attention(query[rows], key[rows], value[rows], group.cu_seqlens_q, scale, output[rows], 0.0)
             continue
         if fused_prefill:
             fused_prefill_attention(

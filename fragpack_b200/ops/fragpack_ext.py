@@ -113,6 +113,8 @@ _SIGNATURES = {
                              c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_ptr, c_ptr],
     "fp_prompt_attention": [c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i32,
                             c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32, c_f32, c_ptr],
+    "fp_prompt_attention_lag": [c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i32,
+                                c_i64, c_ptr, c_i64, c_i64, c_i32, c_i32, c_f32, c_f32, c_ptr],
     "fp_prompt_status": [c_ptr],
     "fp_norm_rotary": [c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_i64, c_ptr, c_f32, c_ptr],
     "fp_hbm_append": [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_ptr,

@@ -278,6 +278,16 @@ int fp_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const vo
                         void* out, int64_t o_token, int64_t o_head, int32_t kv_heads, int32_t group,
                         float scale, void* stream);
 
+/* The same with the choice of the precision of the weights: `lag` (0 .. 8, in powers
+ * of two; 8 above) is how far a row's largest score may rise above the reference
+ * point of its BF16 weights before that follows.  0 makes the largest weight an
+ * exact 1, as in fp_prefill_attention, and is slower. */
+int fp_prompt_attention_lag(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                            int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                            int64_t v_head, const int32_t* starts, int32_t prompts, int64_t tokens,
+                            void* out, int64_t o_token, int64_t o_head, int32_t kv_heads,
+                            int32_t group, float scale, float lag, void* stream);
+
 /* Copies the prompt kernel's status word to the host (synchronises the device, so
  * that every call made before it has reported) and clears it. */
 int fp_prompt_status(int32_t* status);

@@ -5,6 +5,8 @@ Tolerances are those of ``test_gpu_prompt_attention.py`` where nothing else is s
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -165,3 +167,40 @@ def test_status_of_a_call_on_another_stream() -> None:
         check(extension().fp_debug_wait_limit(0, -1))
     torch.cuda.synchronize()
     assert prompt_status() == 0
+
+
+@pytest.mark.parametrize("h,group", [(1, 8), (2, 2)])
+def test_the_caller_chooses_the_precision_of_the_weights(h, group) -> None:
+    """The largest weight is an exact 1 at lag 0; at the default it may be one that BF16 has to round.
+
+    Key 0 has the score 0 and key 200 that of a weight of 128.5, halfway between two BF16 values: relative to the first
+    key tile's maximum its rounding is off by 2^-8, relative to its own by nothing, and key 0's weight of 1 / 128.5 is
+    off by 2^-8 of that.  All other keys are 2^-60 of key 0 and vanish.
+    """
+    n = 900
+    q, k, v = _inputs(n, h, group, seed=25)
+    log2_score = 16.0 * SCALE * 1.4426950408889634  # of a key's dim 0 or 1, in powers of two
+    q[:], k[:] = 0.0, 0.0
+    q[..., :2] = 16.0
+    k[..., 0] = -60.0 / log2_score
+    score = math.log2(128.5) / log2_score
+    k[0, :, 0], k[200, :, 0] = 0.0, score
+    k[200, :, 1] = score - float(k[200, 0, 0])
+    want, _ = _reference(q, k, v, [n])
+    error = {}
+    for lag in (0.0, 8.0):
+        out = torch.zeros_like(q)
+        prompt_attention(q, k, v, _starts([n]), SCALE, out, lag)
+        _check(out, _reference(q, k, v, [n]), n)
+        error[lag] = (out.double() - want)[200:]
+    v0, v200 = (v[t].repeat_interleave(group, 0).double().abs() for t in (0, 200))
+    # The result's rounding, key 0's weight's, and FP32 scores and exponentials (as in _reference).
+    assert bool((error[0.0].abs() <= 2.0**-8 * want[200:].abs() + 2.0**-8 * v0 / 128.5 + 2.0**-10 * (v200 + v0 / 128.5)).all())
+    assert float(error[8.0].square().mean()) > 2.0 * float(error[0.0].square().mean())
+
+
+@pytest.mark.parametrize("lag", [-1.0, 8.5, float("nan"), float("inf")])
+def test_impossible_lags_are_refused(lag) -> None:
+    q, k, v = _inputs(20, 2, 4)
+    with pytest.raises(RuntimeError, match="lag"):
+        prompt_attention(q, k, v, _starts([20]), SCALE, torch.empty_like(q), lag)
