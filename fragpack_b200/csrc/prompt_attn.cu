@@ -1129,7 +1129,9 @@ int fp_prompt_attention_lag(const void* q, int64_t q_token, int64_t q_head, cons
   FP_REQUIRE(prompts > 0 && tokens > 0 && tokens < (1LL << 30) && kv_heads > 0 && kv_heads <= 65535,
              "bad prompt geometry (%d prompts, %lld tokens, %d KV heads)", prompts, (long long)tokens, kv_heads);
   FP_REQUIRE(group == 1 || group == 2 || group == 4 || group == 8, "query group %d must be 1, 2, 4 or 8", group);
-  FP_REQUIRE(scale > 0.f && scale < INFINITY, "the softmax scale must be positive and finite");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  FP_REQUIRE(scale_log2 >= FLT_MIN && scale_log2 < INFINITY,
+             "the softmax scale must be positive and finite, and so must its product with log2(e) in normal FP32");
   FP_REQUIRE(lag >= 0.f && lag <= kLongestLag, "the lag must be within 0 .. %g", kLongestLag);
   FP_REQUIRE(q && k && v && starts && out, "null prompt attention argument");
   const int q_heads = kv_heads * group;
@@ -1155,7 +1157,7 @@ int fp_prompt_attention_lag(const void* q, int64_t q_token, int64_t q_head, cons
   p.head_chunk = head_chunk(tokens, kv_heads);
   p.group = group;
   p.group_log2 = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.lag = lag;
   p.wait_limit = (uint32_t)std::min<long long>(wait_debug().limit, 0xf0000000LL);
   p.skip_tile = (int)std::max<long long>(-1, std::min<long long>(wait_debug().skip_record, 1 << 20));

@@ -45,7 +45,7 @@ def prompt_attention(
             tensors may be strided by 16-byte multiples.
         starts: int32 ``[R + 1]`` first row of each prompt, non-decreasing;
             entries are clamped to ``0 .. T``.
-        scale: Softmax scale, positive.
+        scale: Softmax scale, positive (times log2(e) a normal FP32 number).
         out: BF16 ``[T, H * G, 128]`` output; must not overlap the inputs.
         lag: Precision of the BF16 weights, 0 to ``LONGEST_LAG``: how far (in
             powers of two) a row's largest score may rise above the reference

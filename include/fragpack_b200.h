@@ -268,7 +268,7 @@ int fp_prefill_attention(const void* q, int64_t q_stride, const int64_t* rec_add
  *   starts      int32 [prompts + 1], non-decreasing, within 0 .. tokens; rows
  *               outside are neither attended nor written
  *   group       query heads per KV head: 1, 2, 4 or 8
- *   scale       softmax scale, > 0
+ *   scale       softmax scale, > 0; scale * log2(e) a normal FP32 number
  * Its device-side waits are bounded; should one run out, bit 0 of the status
  * word read by fp_prompt_status is set (the outputs are then invalid).
  */
