@@ -34,6 +34,7 @@ from fragpack_b200.ops.fragpack_ext import (
 )
 
 HEAD_DIM = 128
+_BF16, _FP32, _INT64, _INT32 = torch.bfloat16, torch.float32, torch.int64, torch.int32
 
 
 def rotary_frequencies(
@@ -110,14 +111,36 @@ class Rotary:
         interleaved: Pairs are dims ``(2 i, 2 i + 1)`` instead of
             ``(i, i + rot_dim / 2)``.
         factor: Multiplies the rotated dims.
+
+    Raises:
+        ValueError: For rotated dims out of range or without their turns.
     """
 
     turns: torch.Tensor
     rot_dim: int
     interleaved: bool
     factor: float
-    _native: FpRotary = field(repr=False, compare=False)
-    _ref: Any = field(repr=False, compare=False)  # by reference, made once
+    _native: FpRotary = field(init=False, repr=False, compare=False)
+    _ref: Any = field(init=False, repr=False, compare=False)  # by reference, made once
+
+    def __post_init__(self) -> None:
+        _check_rot_dim(self.rot_dim)
+        turns = self.turns
+        if turns.dtype is not _INT64 or turns.dim() != 1 or not turns.is_contiguous() or len(turns) < self.rot_dim // 2:
+            raise ValueError(f"turns must be contiguous int64 [{self.rot_dim // 2}], not {turns.dtype} {tuple(turns.shape)}")
+        native = FpRotary(turns=turns.data_ptr(), rot_dim=self.rot_dim, interleaved=int(bool(self.interleaved)),
+                          factor=self.factor)
+        object.__setattr__(self, "_native", native)
+        object.__setattr__(self, "_ref", byref(native))
+
+    def __reduce__(self) -> tuple[Any, ...]:
+        # Copies and pickles describe their own tensor.
+        return Rotary, (self.turns, self.rot_dim, self.interleaved, self.factor)
+
+
+def _check_rot_dim(rot_dim: int) -> None:
+    if rot_dim < 0 or rot_dim > HEAD_DIM or rot_dim % 8:
+        raise ValueError(f"rotated dims {rot_dim} must be a multiple of 8 up to {HEAD_DIM}")
 
 
 def make_rotary(
@@ -144,8 +167,7 @@ def make_rotary(
     Raises:
         ValueError: For impossible parameters.
     """
-    if rot_dim < 0 or rot_dim > HEAD_DIM or rot_dim % 8:
-        raise ValueError(f"rotated dims {rot_dim} must be a multiple of 8 up to {HEAD_DIM}")
+    _check_rot_dim(rot_dim)
     if frequencies is None:
         freq, rule_factor = rotary_frequencies(rot_dim, base, scaling)
     else:
@@ -160,11 +182,7 @@ def make_rotary(
     fractions = [int(f / (2.0 * math.pi) * 2.0**64) % (1 << 64) for f in freq.tolist()]
     bits = np.array(fractions + [0] * (not fractions), dtype=np.uint64).view(np.int64)
     turns = torch.from_numpy(bits).to(device)
-    native = FpRotary(turns=turns.data_ptr(), rot_dim=rot_dim, interleaved=int(bool(interleaved)), factor=factor)
-    return Rotary(turns, rot_dim, bool(interleaved), factor, native, byref(native))
-
-
-_BF16, _FP32, _INT64, _INT32 = torch.bfloat16, torch.float32, torch.int64, torch.int32
+    return Rotary(turns, rot_dim, bool(interleaved), factor)
 
 
 # These checks are most of a small call's host time, so the sound case takes one

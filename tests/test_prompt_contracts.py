@@ -2,9 +2,16 @@
 
 from __future__ import annotations
 
+import copy
+import ctypes
+from dataclasses import replace
+import pickle
+
 import pytest
+import torch
 
 from fragpack_b200.ops.fragpack_ext import extension
+from fragpack_b200.ops.rotary import make_rotary
 
 
 @pytest.mark.parametrize("scale", [3e38, 7e-39, 2.0**-140])
@@ -13,3 +20,33 @@ def test_scales_whose_powers_of_two_leave_the_range_are_refused(scale) -> None:
     lib, at = extension(), 1 << 20
     code = lib.fp_prompt_attention(at, 1024, 128, at, 256, 128, at, 256, 128, at, 1, 4, at, 1024, 128, 2, 4, scale, None)
     assert code == -1 and "scale" in lib.fp_last_error().decode()
+
+
+def _described(rotary):
+    native = rotary._native
+    return native.turns, native.rot_dim, native.interleaved, native.factor
+
+
+def test_a_rotary_describes_what_it_says() -> None:
+    """Also one that was derived from another by replacing fields, copied or pickled."""
+    rotary = make_rotary(torch.device("cpu"), 64, interleaved=True)
+    other = make_rotary(torch.device("cpu"), 128)
+    derived = [
+        replace(rotary, factor=2.0), replace(rotary, interleaved=False), replace(rotary, rot_dim=32),
+        replace(rotary, turns=other.turns, rot_dim=128), copy.copy(rotary), copy.deepcopy(rotary),
+        pickle.loads(pickle.dumps(rotary)),
+    ]
+    for x in derived:
+        assert _described(x) == (x.turns.data_ptr(), x.rot_dim, x.interleaved, x.factor)
+        assert ctypes.addressof(x._ref._obj) == ctypes.addressof(x._native)
+    assert derived[0].factor == 2.0 and not derived[1].interleaved and derived[2].rot_dim == 32
+    for x in derived[4:]:
+        assert torch.equal(x.turns, rotary.turns) and (x.rot_dim, x.interleaved, x.factor) == (64, True, 1.0)
+
+
+def test_a_rotary_without_its_turns_is_refused() -> None:
+    rotary = make_rotary(torch.device("cpu"), 64)
+    for wrong in (dict(rot_dim=72), dict(rot_dim=12), dict(rot_dim=136), dict(rot_dim=-8), dict(turns=rotary.turns[:31]),
+                  dict(turns=rotary.turns.int()), dict(turns=torch.zeros(64, dtype=torch.int64)[::2])):
+        with pytest.raises(ValueError):
+            replace(rotary, **wrong)
