@@ -7,10 +7,12 @@
 //   (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t),  t = position * frequency_i
 //
 // Everything between the load and the one rounding of the result to BF16 is
-// FP32.  The angle is reduced exactly: a frequency is held in turns per token
+// FP32.  The angle is reduced in 64 bits: a frequency is held in turns per token
 // as a 64-bit binary fraction, so position * frequency modulo one turn is one
-// wrapping 64-bit multiplication (error: position * 2^-65 turns, at any
-// position), and sine and cosine of the remaining half turn come from the
+// wrapping 64-bit multiplication, which adds no error.  The fraction itself is as
+// good as the double that it comes from (within 2^-54 turns per token for up to
+// one radian per token: 2^-37 turns at position 131,072).  Sine and cosine of the
+// remaining half turn come from the
 // special-function unit, whose absolute error of about 2^-21 there is a 4000th
 // of the half step of the BF16 result.  No table of angles is read.
 //

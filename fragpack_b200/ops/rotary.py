@@ -9,8 +9,10 @@ the reference's, ``fragpack/integrations/vllm/backend.py:504-579``);
 has no counterpart: its engine rotates before the backend is called.
 
 A :class:`Rotary` holds the frequencies in turns per token as 64-bit binary
-fractions, so that ``position * frequency`` modulo one turn is exact at any
-position and no table of angles is kept.
+fractions: ``position * frequency`` modulo one turn is one integer product,
+which adds no error at any position, and no table of angles is kept.  The
+fractions are as good as float64 frequencies: within 2**-54 turns per token up
+to one radian per token.
 """
 
 from __future__ import annotations

@@ -5,6 +5,7 @@ from __future__ import annotations
 import copy
 import ctypes
 from dataclasses import replace
+from decimal import Decimal, localcontext
 import pickle
 
 import pytest
@@ -50,3 +51,15 @@ def test_a_rotary_without_its_turns_is_refused() -> None:
                   dict(turns=rotary.turns.int()), dict(turns=torch.zeros(64, dtype=torch.int64)[::2])):
         with pytest.raises(ValueError):
             replace(rotary, **wrong)
+
+
+@pytest.mark.parametrize("rot_dim,base", [(128, 10000.0), (64, 500000.0), (96, 1000000.0), (8, 2.0)])
+def test_turns_are_within_the_stated_bound_of_the_exact_ones(rot_dim, base) -> None:
+    """2^-54 turns per token (see csrc/rotary.cu), against 60-digit decimal arithmetic."""
+    with localcontext() as context:
+        context.prec = 60
+        pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+        for i, bits in enumerate(make_rotary(torch.device("cpu"), rot_dim, base).turns.tolist()):
+            frequency = (-Decimal(2 * i) / Decimal(rot_dim) * Decimal(base).ln()).exp()
+            exact = frequency / (2 * pi)
+            assert abs(Decimal(bits % 2**64) / Decimal(2**64) - exact) <= Decimal(2) ** -54
