@@ -12,9 +12,9 @@
 // wrapping 64-bit multiplication, which adds no error.  The fraction itself is as
 // good as the double that it comes from (within 2^-54 turns per token for up to
 // one radian per token: 2^-37 turns at position 131,072).  Sine and cosine of the
-// remaining half turn come from the
-// special-function unit, whose absolute error of about 2^-21 there is a 4000th
-// of the half step of the BF16 result.  No table of angles is read.
+// remaining half turn come from the special-function unit, whose absolute error
+// of about 2^-21 there is a 4000th of the half step of the BF16 result.  No table
+// of angles is read.
 //
 // A head's 128 values are held by half a warp: a lane has two pieces of four
 // neighbouring dims, half a rotated range apart, so that both members of every
@@ -449,13 +449,14 @@ int rotary_params(RotaryParams& p, const fp_heads* q, const fp_heads* k, const v
 // which is 0.91 of the measured copy bandwidth.
 template <bool kAppend>
 int launch_rows(RotaryParams& p, const StoreView& v, bool interleaved, cudaStream_t stream) {
-  const bool many = p.tokens * (p.q.heads + p.k.heads) >= kManyRows;
+  // An append has too few tokens here (kFewTokens) for the second form.
+  const bool many = !kAppend && p.tokens * (p.q.heads + p.k.heads) >= kManyRows;
   p.unit = many ? 16 : 2;
   const int64_t units = (p.q.heads + p.unit - 1) / p.unit + (kAppend ? 2LL : 1LL) * ((p.k.heads + p.unit - 1) / p.unit);
   FP_REQUIRE(units <= 65535, "too many heads (%d + %d)", p.q.heads, p.k.heads);
-  const auto kernel = interleaved ? many ? rotary_rows_kernel<kAppend, true, 4> : rotary_rows_kernel<kAppend, true, 2>
-                      : many      ? rotary_rows_kernel<kAppend, false, 4>
-                                  : rotary_rows_kernel<kAppend, false, 2>;
+  auto kernel = interleaved ? rotary_rows_kernel<kAppend, true, 2> : rotary_rows_kernel<kAppend, false, 2>;
+  if constexpr (!kAppend)
+    if (many) kernel = interleaved ? rotary_rows_kernel<false, true, 4> : rotary_rows_kernel<false, false, 4>;
   constexpr int per_block = kRowThreads / 16;
   kernel<<<dim3((unsigned)((p.tokens + per_block - 1) / per_block), (unsigned)units), kRowThreads, 0, stream>>>(p, v);
   FP_LAUNCH_CHECK("rotary_rows_kernel");
