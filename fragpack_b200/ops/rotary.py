@@ -71,7 +71,7 @@ def rotary_frequencies(
     Raises:
         ValueError: For an unknown rule or impossible parameters.
     """
-    if rot_dim < 0 or rot_dim % 2 or base <= 1.0:
+    if rot_dim < 0 or rot_dim % 2 or not 1.0 < base < math.inf:
         raise ValueError(f"rotated dims {rot_dim} must be even and the base {base} above 1")
     freq = base ** (-np.arange(0, rot_dim, 2, dtype=np.float64) / max(rot_dim, 1))
     if scaling is None:
@@ -79,11 +79,17 @@ def rotary_frequencies(
     rule, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
     if rule not in ("linear", "bands", "ramp"):
         raise ValueError(f"unknown rotary scaling {rule!r}")
-    if not factor >= 1.0:
+    if not 1.0 <= factor < math.inf:
         raise ValueError(f"rotary scaling needs a factor of at least 1, not {factor}")
     if rule == "linear":
         return freq / factor, 1.0
+    needed = ("original", "low_freq_factor", "high_freq_factor") if rule == "bands" else ("original",)
+    missing = [name for name in needed if name not in scaling]
+    if missing:
+        raise ValueError(f"rotary scaling {rule!r} needs {', '.join(missing)}")
     original = float(scaling["original"])
+    if not 0.0 < original < math.inf:
+        raise ValueError(f"rotary scaling needs an original context above 0, not {original}")
     if rule == "bands":
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
         if not high > low:
@@ -95,8 +101,11 @@ def rotary_frequencies(
     def pair_turning(times: float) -> float:
         return rot_dim * math.log(original / (2.0 * math.pi * times)) / (2.0 * math.log(base))
 
-    first = max(math.floor(pair_turning(float(scaling.get("beta_fast", 32.0)))), 0)
-    last = min(math.ceil(pair_turning(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    beta_fast, beta_slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not 0.0 < beta_slow <= beta_fast < math.inf:
+        raise ValueError(f"a rotary ramp needs beta_fast {beta_fast} of at least beta_slow {beta_slow}, which is above 0")
+    first = max(math.floor(pair_turning(beta_fast)), 0)
+    last = min(math.ceil(pair_turning(beta_slow)), rot_dim - 1)
     ramp = np.clip((np.arange(rot_dim // 2) - first) / max(last - first, 1e-3), 0.0, 1.0)
     attention = float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
     return freq * (1.0 - ramp) + freq / factor * ramp, attention
@@ -180,6 +189,8 @@ def make_rotary(
         if freq.shape != (rot_dim // 2,) or not np.isfinite(freq).all():
             raise ValueError(f"frequencies must be {rot_dim // 2} finite numbers")
     factor = float(rule_factor if factor is None else factor)
+    if not math.isfinite(factor):
+        raise ValueError(f"the factor on the rotated dims must be finite, not {factor}")
     # The fraction of a turn per token; whole turns per token change nothing.
     fractions = [int(f / (2.0 * math.pi) * 2.0**64) % (1 << 64) for f in freq.tolist()]
     bits = np.array(fractions + [0] * (not fractions), dtype=np.uint64).view(np.int64)

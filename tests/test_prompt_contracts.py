@@ -63,3 +63,25 @@ def test_turns_are_within_the_stated_bound_of_the_exact_ones(rot_dim, base) -> N
             frequency = (-Decimal(2 * i) / Decimal(rot_dim) * Decimal(base).ln()).exp()
             exact = frequency / (2 * pi)
             assert abs(Decimal(bits % 2**64) / Decimal(2**64) - exact) <= Decimal(2) ** -54
+
+
+BANDS = {"type": "bands", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original": 8192}
+RAMP = {"type": "ramp", "factor": 4.0, "original": 4096}
+
+
+@pytest.mark.parametrize("scaling", [
+    {k: x for k, x in BANDS.items() if k != "original"}, {k: x for k, x in BANDS.items() if k != "low_freq_factor"},
+    {k: x for k, x in BANDS.items() if k != "high_freq_factor"}, {k: x for k, x in RAMP.items() if k != "original"},
+    {**RAMP, "original": 0}, {**BANDS, "original": -1}, {**RAMP, "beta_slow": 0.0}, {**RAMP, "beta_fast": 0.5},
+    {"type": "linear", "factor": float("inf")}, {**RAMP, "beta_fast": float("nan")},
+    {**RAMP, "attention_factor": float("nan")},
+])
+def test_scalings_without_a_meaning_are_refused(scaling) -> None:
+    with pytest.raises(ValueError):
+        make_rotary(torch.device("cpu"), 64, 10000.0, scaling=scaling)
+
+
+def test_bases_and_factors_that_are_no_numbers_are_refused() -> None:
+    for wrong in (dict(base=float("nan")), dict(base=float("inf")), dict(factor=float("nan")), dict(factor=float("-inf"))):
+        with pytest.raises(ValueError):
+            make_rotary(torch.device("cpu"), 64, **wrong)
