@@ -538,23 +538,15 @@ __device__ __forceinline__ void clear_value_rows(uint8_t* tile, int from, int la
 __device__ __forceinline__ bool has_stray_values(const uint8_t* tile, int from, int to, int lane) {
   uint32_t sum[4] = {0, 0, 0, 0};  // 0 * x of everything, as pairs
 #pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    const uint4* const rows = reinterpret_cast<const uint4*>(tile + half * kKeyHalf) + 8 * from;
-    const int count = 8 * (to - from);
-#pragma unroll 1
-    for (int i = lane; i < count; i += 4 * 32) {
-      uint4 x[4];
+  for (int i = 8 * from + lane; i < 8 * to; i += 32)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = i + 32 * u < count ? rows[i + 32 * u] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(x[u].x), "r"(0u));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(x[u].y), "r"(0u));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(x[u].z), "r"(0u));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(x[u].w), "r"(0u));
-      }
+    for (int half = 0; half < 2; ++half) {
+      const uint4 x = reinterpret_cast<const uint4*>(tile + half * kKeyHalf)[i];
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(x.x), "r"(0u));
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(x.y), "r"(0u));
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(x.z), "r"(0u));
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(x.w), "r"(0u));
     }
-  }
   return __any_sync(0xffffffffu, (sum[0] | sum[1] | sum[2] | sum[3]) != 0);
 }
 
@@ -645,6 +637,7 @@ __device__ __forceinline__ void issue_values(PromptSmem& sm, uint32_t tmem, int 
       if (from < to && has_stray_values(sm.v[stage], from, to, lane)) {
         // What is noted of an earlier item has been read once its O has been: of the
         // tiles that this item has, that is so from its second key tile on.
+#pragma unroll 1
         for (int t = 0; t < kQTiles; ++t)
           if ((j == 0 || w.last[t] < 0) && items[t] > 0) await(&sm.o_free[t], (items[t] - 1) & 1u, &sm.wait);
         screen_values(sm, sm.v[stage], j * kKeys, !screened, lane);
