@@ -121,6 +121,16 @@ def test_values_of_the_largest_size() -> None:
     _check(out, _reference(q, k, v, lens), sum(lens))
 
 
+def test_values_of_a_small_size() -> None:
+    """2^-85, in prompts of up to 3,000 tokens: as accurate as others."""
+    lens = [1, 90, 3000, 5]
+    q, k, v = _inputs(sum(lens), 2, 4, seed=26)
+    v = (v.float() * 2.0**-85).to(torch.bfloat16)
+    out = torch.zeros_like(q)
+    prompt_attention(q, k, v, _starts(lens), SCALE, out)
+    _check(out, _reference(q, k, v, lens), sum(lens))
+
+
 def test_one_infinity_in_a_very_long_prompt() -> None:
     n = 140_000
     q, k, v = _inputs(n, 1, 8, seed=23)
