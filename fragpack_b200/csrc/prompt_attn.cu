@@ -20,20 +20,24 @@
 // while the softmax works on these; a tile's chain is then the softmax alone, and
 // the tensor cores follow.  That is why a key tile is narrower than 128: with 128
 // keys P has to lie over its S, every tile waits for softmax, O product and S
-// product in turn, and one prompt of 32,768 tokens (8 + 1 heads) took 2,046 us
-// against 1,667.
+// product in turn, and an earlier form of this kernel took 23 % longer on one
+// prompt of 32,768 tokens (8 + 1 heads).
 //
 // What bounds it: an S product of 128 rows takes eight steps of 52 cycles (32 +
 // 80 / 4 each, the 32 whatever the width), an O product five of 64; that is 736
-// cycles where the arithmetic alone is 640, so the products reach at most
-// 0.87 of the tensor cores' rate.  Measured: 1,381 TFLOP/s in short runs on that
-// prompt (1,592 us, 0.84 of 1,643), 1,170 to 1,210 without a pause, where the
-// card's power limit holds the clock near 1.4 GHz (0.84 to 0.87 of the 1,400 that
-// plain products keep up); 1,158 on 16 prompts of 1,000 to 4,096 tokens (32 + 8
-// heads, 689 us); 48 us for 64 prompts of up to 300 tokens, where an item is too
-// short to hide its own start.  8,192 tokens (32 + 8 heads) under counters: tensor
-// pipe active 68 %, issue slots 44 %, special-function unit about half, 103 MB
-// read from DRAM and 32 MB written (the results stay in L2 for the next reader).
+// cycles where the arithmetic alone is 640.  That prompt has 420,455 such steps of a
+// key tile and a query tile, 1,064 us of products on 148 SMs at 1.965 GHz, and takes
+// 1,600 us in short runs (1,375 TFLOP/s, 0.84 of 1,643): nothing is saturated.
+// 8,192 tokens (32 + 8 heads) under counters: tensor pipe active 67 %, issue slots
+// 44 %, special-function unit about half, 103 MB read from DRAM and 33 MB written
+// (the results stay in L2 for the next reader); a tile's S product, softmax and O
+// product follow one another, and two tiles do not fill the gaps.  Without a pause
+// the power limit holds the clock near 1.4 GHz: 1,160 to 1,210 TFLOP/s (0.83 to 0.86
+// of the 1,400 that plain products keep up).  16 prompts of 1,000 to 4,096 tokens
+// (32 + 8 heads) 702 us, 1,136 TFLOP/s; 64 prompts of up to 300 tokens 48.5 us, where
+// an item is too short to hide its own start.  (Figures here and below are short
+// runs of the present kernel, within 1.5 % from card to card, where nothing else is
+// said.)
 //
 // One CTA per SM at a time, which goes from item to item; its warps meet only
 // through mbarriers, and every wait is bounded and reports through the status
@@ -43,15 +47,15 @@
 //   result warps   divide an item's O by the sums and store it
 //   score warp     issues S products, value warp O products (one elected lane;
 //                  two warps, so that neither waits behind the other's barriers;
-//                  four, one per tile too, polled so much that the same prompt
-//                  took 1,822 us against 1,640)
+//                  four, one per tile too, polled so much that an earlier form
+//                  took 11 % longer)
 //   load warp      loads the items' tiles
 //   item warp      picks the CTA's items, up to two ahead of the others
 //
 // The code is kept short (waits with a small way out, loops over the two tiles
 // rolled in the result warps): sixteen warps in seven roles share the instruction
-// caches, and the same kernel with 64 short prompts took 67 us with the loops
-// unrolled and 53 without.
+// caches, and 64 short prompts take 56.7 us with the loops of the result warps
+// unrolled and 48.5 without.
 #include <cuda.h>
 #include <math.h>
 
@@ -90,10 +94,10 @@ constexpr int kSoftmaxRegs = 184, kResultRegs = 88, kOtherRegs = 56;
 // up to this.  Nothing is lost in range, but the largest weights, rounded to BF16, no
 // longer include the exact 1 of a row's maximum.  RMS error against 64 bits relative to that
 // of attention in FP32 with one rounding (five sets of prompts of 1 to 16,384 tokens),
-// and times of 16 ragged prompts / of one of 32,768 tokens: 8: 1.16 to 1.34, 710 /
-// 1,616 us; 4: 1.15 to 1.22, 794 / 1,680; 2: 1.13 to 1.17, 829 / 1,714; 1: 1.12 to
-// 1.14, 842 / 1,750; 0: 1.08 to 1.12, 859 / 1,835 (a rescale waits for the O product
-// before it).  Largest error at 8: up to 1.9 times that of FP32, at 0 up to 1.2 times.
+// and times of 16 ragged prompts / of one of 32,768 tokens: 8: 1.16 to 1.34, 705 /
+// 1,612 us; 4: 1.15 to 1.22, 782 / 1,672; 1: 1.12 to 1.14, 830 / 1,739; 0: 1.08 to
+// 1.12, 844 / 1,814 (a rescale waits for the O product before it).  Largest error at
+// 8: up to 1.9 times that of FP32, at 0 up to 1.2 times.
 constexpr float kLongestLag = 8.f;
 
 __device__ int32_t g_prompt_status;
@@ -182,7 +186,7 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, PromptWait
 
 // The same with one answer for all lanes of a warp, so that none leaves a loop alone
 // when a wait gives up.  Once per item: with votes in all waits one prompt of 32,768
-// tokens (8 + 1 heads) took 1,798 us against 1,592.
+// tokens (8 + 1 heads) takes 13 % longer.
 __device__ __forceinline__ bool await_all(uint64_t* bar, uint32_t parity, PromptWait* ws) {
   return __all_sync(0xffffffffu, await(bar, parity, ws));
 }
@@ -389,8 +393,8 @@ struct ItemPicker {
 // that whoever is done first goes on first.  The next block is asked for once the
 // load warp has begun with the last one taken and the result warps with the one
 // before: asked for earlier, it would be bound to a CTA that may be late (two
-// prompts of 8,192 tokens, 32 + 32 heads: 930 us without the wait for the load
-// warp, 899 with it; without a pause 1,051 / 1,029).  Blocks come in rising order
+// prompts of 8,192 tokens, 32 + 32 heads: 914 us without the wait for the load
+// warp, 888 with it).  Blocks come in rising order
 // as a rule, but nothing promises it: whatever order they come in, every one is
 // looked at, also behind one that has no item.
 __device__ __forceinline__ void ask_for_block(PromptSmem& sm, int lane) {
@@ -768,7 +772,7 @@ __device__ __forceinline__ void prompt_softmax(const PromptParams& p, PromptSmem
   // turns at the exponentials, tile 0 first: side by side both would be slow,
   // and the tensor cores would wait for both.  The turn is passed on at half of
   // them, so that the other's are there when these end (one prompt of 32,768
-  // tokens, 8 + 1 heads: 1,592 us, at the end 1,608, at a third 1,605).
+  // tokens, 8 + 1 heads: 1,601 us, at the end or at a third 1,613).
   uint32_t turns = 0;
   const auto take_turn = [&] {
     await(&sm.turn[mine][rows], (turns + (uint32_t)mine + 1) & 1u, &sm.wait);  // tile 0's first passes at once
@@ -1079,9 +1083,9 @@ int head_map(CUtensorMap& map, const char* name, const void* base, int64_t token
 // as kChunkBytes hold, so that they stay in L2 while every pair of query tiles
 // reads them; rather fewer than chunks of different sizes, whose last one would
 // leave SMs without work.  All heads at a time / 20 / 32 / 48 / 64 / 96 MB: 16
-// prompts of 1,000 to 4,096 tokens (32 + 8 heads, 168 MB) 748 / 709 / 709 / 695 /
-// 697 / 708 us, two of 8,192 (32 + 32 heads, 268 MB) 956 / 959 / 935 / 960 / 914
-// / 925 us.
+// prompts of 1,000 to 4,096 tokens (32 + 8 heads, 168 MB) 748 / 710 / 709 / 700 /
+// 701 / 706 us, two of 8,192 (32 + 32 heads, 268 MB) 953 / 924 / 897 / 897 / 888
+// / 889 us.
 int head_chunk(int64_t tokens, int kv_heads) {
   const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kv_heads, kChunkBytes / (tokens * 512)));
   for (int n = most; 2 * n > most; --n)

@@ -54,7 +54,7 @@ def prompt_attention(
             point of its weights before that follows.  At 0 the largest weight
             is an exact 1, as in ``prefill_attention``; the RMS error is then
             1.08 to 1.12 times that of FP32 attention rounded once, against
-            1.16 to 1.34 at the default, and a call takes 3 to 21 % longer.
+            1.16 to 1.34 at the default, and a call takes 1 to 20 % longer.
 
     Raises:
         ValueError: If the query group does not divide ``GQA``.
