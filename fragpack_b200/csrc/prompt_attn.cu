@@ -91,13 +91,13 @@ static_assert(kTmemP + kQTiles * kKeys / 2 <= kTmemColumns && kKeys % 16 == 0, "
 constexpr int kSoftmaxRegs = 184, kResultRegs = 88, kOtherRegs = 56;
 // How far (log2 units) a row's maximum may rise above the reference point of its
 // exponentials before the reference follows and O is rescaled: the caller's choice,
-// up to this.  Nothing is lost in range, but the largest weights, rounded to BF16, no
-// longer include the exact 1 of a row's maximum.  RMS error against 64 bits relative to that
-// of attention in FP32 with one rounding (five sets of prompts of 1 to 16,384 tokens),
-// and times of 16 ragged prompts / of one of 32,768 tokens: 8: 1.16 to 1.34, 705 /
-// 1,612 us; 4: 1.15 to 1.22, 782 / 1,672; 1: 1.12 to 1.14, 830 / 1,739; 0: 1.08 to
-// 1.12, 844 / 1,814 (a rescale waits for the O product before it).  Largest error at
-// 8: up to 1.9 times that of FP32, at 0 up to 1.2 times.
+// up to this.  Nothing is lost in range, but the largest weights, rounded to BF16,
+// no longer include the exact 1 of a row's maximum.  RMS error against 64 bits,
+// relative to that of attention in FP32 with one rounding (five sets of prompts of 1
+// to 16,384 tokens), and times of 16 ragged prompts / of one of 32,768 tokens: 8:
+// 1.16 to 1.34, 705 / 1,612 us; 4: 1.15 to 1.22, 782 / 1,672; 1: 1.12 to 1.14, 830 /
+// 1,739; 0: 1.08 to 1.12, 844 / 1,814 (a rescale waits for the O product before it).
+// Largest error at 8: up to 1.9 times that of FP32, at 0 up to 1.2 times.
 constexpr float kLongestLag = 8.f;
 
 __device__ int32_t g_prompt_status;
@@ -394,9 +394,9 @@ struct ItemPicker {
 // load warp has begun with the last one taken and the result warps with the one
 // before: asked for earlier, it would be bound to a CTA that may be late (two
 // prompts of 8,192 tokens, 32 + 32 heads: 914 us without the wait for the load
-// warp, 888 with it).  Blocks come in rising order
-// as a rule, but nothing promises it: whatever order they come in, every one is
-// looked at, also behind one that has no item.
+// warp, 888 with it).  Blocks come in rising order as a rule, but nothing promises
+// it: whatever order they come in, every one is looked at, also behind one that has
+// no item.
 __device__ __forceinline__ void ask_for_block(PromptSmem& sm, int lane) {
   if (lane == 0) {
     mbar_expect_tx(&sm.block_full, 16);
@@ -554,10 +554,10 @@ __device__ __forceinline__ bool has_stray_values(const uint8_t* tile, int from, 
   return __any_sync(0xffffffffu, (sum[0] | sum[1] | sum[2] | sum[3]) != 0);
 }
 
-// Takes all of the tile's out of it (they become zero) and notes in sm.stray, per dim, the
-// first token of the prompt that holds an infinity of either sign and the first
-// that holds a NaN; the result warps bring them back into the rows that see these
-// tokens.  So such values take no time beside the search, which costs 64 short
+// Takes all of the tile's out of it (they become zero) and notes in sm.stray, per
+// dim, the first token of the prompt that holds an infinity of either sign and the
+// first that holds a NaN; the result warps bring them back into the rows that see
+// these tokens.  So such values take no time beside the search, which costs 64 short
 // prompts 1 us (47.5 to 48.4) and 16 ragged ones 1 %; rows that came out NaN computed
 // again one by one took 600 times as long where a prompt of 4,096 tokens held an
 // infinity in its first token.  `fresh`: the first time in this item.

@@ -37,9 +37,9 @@ def prompt_attention(
     tensors; each of its rows sees the prompt's rows up to and including
     itself.  Rows outside every prompt are left as they were, and what they
     hold reaches no result.  Infinities and NaN reach the rows that see them and
-    no others, and take no more time than other values.  Values up to BF16's
-    largest are summed in range; those below about 2**-85 lose bits, as weighted sums
-    start at 2**-126.
+    no others, and those of ``v`` take no more time than other values.  Values up
+    to BF16's largest are summed in range; those below about 2**-85 lose bits, as
+    weighted sums start at 2**-126.
 
     Args:
         q: BF16 ``[T, H * G, 128]`` queries.

@@ -7,10 +7,13 @@ import ctypes
 from dataclasses import replace
 from decimal import Decimal, localcontext
 import pickle
+from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
+from fragpack_b200.integrations.vllm import backend
 from fragpack_b200.ops.fragpack_ext import extension
 from fragpack_b200.ops.rotary import make_rotary
 
@@ -85,3 +88,21 @@ def test_bases_and_factors_that_are_no_numbers_are_refused() -> None:
     for wrong in (dict(base=float("nan")), dict(base=float("inf")), dict(factor=float("nan")), dict(factor=float("-inf"))):
         with pytest.raises(ValueError):
             make_rotary(torch.device("cpu"), 64, **wrong)
+
+
+def test_run_layer_attends_over_prompts_with_the_most_precise_weights(monkeypatch) -> None:
+    """As the attention over records, which it replaces: a lag of 0."""
+    calls = []
+    monkeypatch.setattr(backend, "prompt_attention", lambda *args: calls.append(args))
+    table, none = torch.arange(20, dtype=torch.int32).view(2, 10), torch.zeros(0)
+    groups = backend.plan_prefill_groups(table, 0, 2, np.array([0, 7, 12]), np.array([7, 5]), 100, torch.device("cpu"),
+                                         split_whole=True)
+    store = SimpleNamespace(write=lambda *a: None, encode=lambda *a: None, commit=lambda: None)
+    md = backend.FragPackMetadata(
+        store=store, layer_tables=[None], layer_index={}, last_layer=0, slot_mapping=torch.arange(12), num_tokens=12,
+        num_decodes=0, decode_block_table=none, decode_seq_lens=none, units=1, decode_workspace=(none,) * 3,
+        max_close=0, prefills=groups, wk=none, wv=none, prompt_attention=True,
+    )
+    q = torch.zeros(12, 8, 128, dtype=torch.bfloat16)
+    backend.run_layer(md, 0, q, q[:, :2], q[:, :2], q.clone(), 0.1)
+    assert [(args[3].tolist(), args[4], args[6]) for args in calls] == [([0, 7, 12], 0.1, 0.0)]
